@@ -1,0 +1,84 @@
+// Activations fused into group norm, the causal convolution and the selective
+// scan, as functions of the value u before the activation.
+#pragma once
+#include "common.h"
+
+namespace kfb {
+
+// codes of ops/nn.py _FUSED_ACTS
+enum FusedAct : int { ACT_LINEAR = 0, ACT_RELU = 1, ACT_RELU6 = 2, ACT_TANH = 3, ACT_SILU = 4 };
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// v_exp_f32 / v_rcp_f32 are good to about 1 ulp; log2(e) u is rounded once, a
+// relative error of |u| 2^-24 in the exponential and less in the sigmoid.
+__device__ __forceinline__ float sigmoidf(float u) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * u));
+}
+
+// u * sigmoid(u): below about -88 the exponential is infinite and u * 0 = -0,
+// but -inf * 0 would be NaN: the limit is 0.
+__device__ __forceinline__ float siluf(float u) { return u == -INFINITY ? 0.f : u * sigmoidf(u); }
+
+__device__ __forceinline__ float dsiluf(float u) {
+  const float s = sigmoidf(u);
+  if (s == 0.f) return 0.f;  // u (1 - s) s with u = -inf
+  if (u == INFINITY) return 1.f;
+  return s * (1.f + u * (1.f - s));
+}
+
+__device__ __forceinline__ float tanh_f(float u) {
+  // 1 - 2 / (1 + e^{2|u|}); near 0 the odd series, where the difference cancels
+  const float a = fabsf(u);
+  const float e = __builtin_amdgcn_exp2f(2.f * LOG2E * a);
+  const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + e);
+  const float q = a * a;
+  const float small =
+      a * (1.f + q * (-1.f / 3 + q * (2.f / 15 + q * (-17.f / 315 + q * (62.f / 2835)))));
+  return copysignf(a < 0.25f ? small : big, u);
+}
+
+// y = act(u).  ``act`` is uniform over a launch: one scalar branch per call.
+__device__ __forceinline__ float act_fwd(float u, int act) {
+  switch (act) {
+    case ACT_RELU: return u > 0.f || u != u ? u : 0.f;  // NaN stays NaN
+    case ACT_RELU6: return u != u ? u : fminf(fmaxf(u, 0.f), 6.f);
+    case ACT_TANH: return tanh_f(u);
+    case ACT_SILU: return siluf(u);
+    default: return u;
+  }
+}
+
+// dact/du at u; the gradient at the kinks 0 and 6 is 0.
+__device__ __forceinline__ float act_grad(float u, int act) {
+  switch (act) {
+    case ACT_RELU: return u > 0.f ? 1.f : 0.f;
+    case ACT_RELU6: return u > 0.f && u < 6.f ? 1.f : 0.f;
+    case ACT_TANH: {
+      const float t = tanh_f(u);
+      return 1.f - t * t;
+    }
+    case ACT_SILU: return dsiluf(u);
+    default: return 1.f;
+  }
+}
+
+// e^v to about 1.5 ulp for any v: the rounding error of log2(e) v, kept from
+// the fused multiply-add, comes back as a first-order factor.
+__device__ __forceinline__ float exp_f(float v) {
+  const float p = LOG2E * v, lo = fmaf(LOG2E, v, -p) + 1.9259629911e-8f * v;
+  const float e = __builtin_amdgcn_exp2f(p);
+  return fabsf(p) < 126.f ? fmaf(e, LN2 * lo, e) : e;
+}
+
+// log(1 + e^v) = max(v, 0) + log1p(e^-|v|).  log1p(e) = log(w) e / (w - 1) with
+// w = 1 + e rounded (w - 1 is exact): the relative error stays at a few ulp for
+// small e, where log(w) alone loses what the rounding of w drops.
+__device__ __forceinline__ float softplusf(float v) {
+  const float e = exp_f(-fabsf(v));
+  const float w = 1.f + e;
+  const float l = w == 1.f ? e : LN2 * __builtin_amdgcn_logf(w) * e * __builtin_amdgcn_rcpf(w - 1.f);
+  return fmaxf(v, 0.f) + (v != v ? v : l);
+}
+
+}  // namespace kfb

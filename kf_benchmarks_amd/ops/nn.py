@@ -14,6 +14,7 @@ Layouts:
 
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 from typing import Optional, Sequence, Tuple
@@ -568,6 +569,141 @@ def _bn_infer_gpu(x, gamma, beta, residual, rm, rv, eps, relu):
            N.ptr(gamma), N.ptr(beta), rm.data_ptr(), rv.data_ptr(), float(eps),
            coef[0].data_ptr(), coef[1].data_ptr(), int(relu), N.stream(x.device))
     return y
+
+
+# ------------------------------------------------------------------ group norm
+# activations that group norm and ops.ssm apply themselves (csrc/act.h)
+_FUSED_ACTS = {None: 0, "linear": 0, "relu": 1, "relu6": 2, "tanh": 3, "silu": 4}
+
+
+def fused_act_code(kind) -> int:
+    try:
+        return _FUSED_ACTS[kind]
+    except KeyError:
+        raise KeyError("Invalid activation type '%s'" % (kind,)) from None
+
+
+def apply_act(u, kind):
+    """The fused activations in plain PyTorch (CPU path)."""
+    code = fused_act_code(kind)
+    if code == 1:
+        return torch.relu(u)
+    if code == 2:
+        return torch.clamp(u, 0.0, 6.0)
+    if code == 3:
+        return torch.tanh(u)
+    return F.silu(u) if code == 4 else u
+
+
+def check_params(x, shape, **params):
+    """Parameters of an op on ``x``: fp32, contiguous, ``shape``, x's device."""
+    for name, p in params.items():
+        if p is None:
+            continue
+        if p.dtype != torch.float32 or not p.is_contiguous() or tuple(p.shape) != tuple(shape):
+            raise ValueError("%s: a contiguous fp32 tensor of shape %s expected, got %s %s" % (
+                name, tuple(shape), p.dtype, tuple(p.shape)))
+        if p.device != x.device:
+            raise ValueError("%s is on %s, the input on %s" % (name, p.device, x.device))
+
+
+def on_device(x):
+    """Context in which ``x``'s device is the current one (kernels launch on
+    the current device, whatever stream they are given)."""
+    if x.device.index is None or x.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(x.device)
+
+
+N.register_optional("kfb_gn_fwd_ws", [N.I, N.L, N.L, N.I, N.I], N.L)
+N.register_optional("kfb_gn_bwd_ws", [N.I, N.L, N.L, N.I, N.I], N.L)
+N.register_optional("kfb_gn_fwd", [N.I, N.P, N.P, N.L, N.L, N.I, N.I, N.P, N.P, N.F, N.I, N.P, N.P,
+                                   N.P, N.P])
+N.register_optional("kfb_gn_bwd", [N.I, N.P, N.P, N.P, N.L, N.L, N.I, N.I, N.P, N.P, N.I, N.P, N.P,
+                                   N.P, N.P, N.I, N.I, N.P, N.P])
+
+
+def _gn_forward(x, gamma, beta, groups, eps, act):
+    C, n = x.shape[-1], x.shape[0]
+    hw = x.numel() // (n * C)
+    y = torch.empty_like(x)
+    nws = N.query("kfb_gn_fwd_ws", N.dt(x), n, hw, C, groups)
+    st = torch.empty((2 * n * groups + nws,), dtype=torch.float32, device=x.device)
+    base = st.data_ptr()
+    N.call("kfb_gn_fwd", N.dt(x), x.data_ptr(), y.data_ptr(), n, hw, C, groups, N.ptr(gamma),
+           N.ptr(beta), float(eps), act, base, base + 4 * n * groups, base + 8 * n * groups,
+           N.stream(x.device))
+    return y, st
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, groups, eps, act):
+        y, st = _gn_forward(x, gamma, beta, groups, eps, act)
+        ctx.save_for_backward(x, gamma, beta, st)
+        ctx.args = (groups, act)
+        ctx.params = (gamma, beta)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gamma, beta, st = ctx.saved_tensors
+        groups, act = ctx.args
+        dy = dy.contiguous()
+        C, n, dev = x.shape[-1], x.shape[0], x.device
+        hw = x.numel() // (n * C)
+        dx = torch.empty_like(x)
+        sinks = [_grad_sink(p) for p in ctx.params]
+        grads = [s if s is not None or p is None else torch.empty((C,), dtype=torch.float32,
+                                                                  device=dev)
+                 for s, p in zip(sinks, ctx.params)]
+        ws = torch.empty((N.query("kfb_gn_bwd_ws", N.dt(x), n, hw, C, groups),),
+                         dtype=torch.float32, device=dev)
+        base = st.data_ptr()
+        N.call("kfb_gn_bwd", N.dt(x), dy.data_ptr(), x.data_ptr(), dx.data_ptr(), n, hw, C, groups,
+               N.ptr(gamma), N.ptr(beta), act, base, base + 4 * n * groups, N.ptr(grads[0]),
+               N.ptr(grads[1]), int(sinks[0] is not None), int(sinks[1] is not None),
+               ws.data_ptr(), N.stream(dev))
+        for k, p in enumerate(ctx.params):
+            if sinks[k] is not None:
+                _grad_ready(p)
+                grads[k] = None
+        return dx, grads[0], grads[1], None, None, None
+
+
+def group_norm(x, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], groups: int,
+               eps: float = 1e-5, activation: Optional[str] = None):
+    """y = act(gamma (x - mean) / sqrt(var + eps) + beta) over channels-last x
+    [N, ..., C], with the statistics of each image's ``groups`` runs of
+    C / groups channels (all positions between the first and last dim; [N, C]
+    normalises each row's groups).  ``gamma`` / ``beta``: fp32 [C] or None (1 /
+    0).  ``activation``: None / "linear", "relu", "relu6", "tanh", "silu",
+    applied in the same pass.  It needs no batch statistics, so it is the same
+    function in training, in evaluation and for one token.  Differentiable
+    once in x, gamma and beta; the backward recomputes the activation from x."""
+    act = fused_act_code(activation)
+    if x.dim() < 2 or x.numel() == 0:
+        raise ValueError("group_norm: a non-empty [N, ..., C] tensor expected, got %s" %
+                         (tuple(x.shape),))
+    C = x.shape[-1]
+    if groups < 1 or C % groups:
+        raise ValueError("group_norm: %d channels do not split into %d groups" % (C, groups))
+    check_params(x, (C,), gamma=gamma, beta=beta)
+    if not _on_gpu(x):
+        y = x.float().reshape(x.shape[0], -1, groups, C // groups)
+        v, m = torch.var_mean(y, dim=(1, 3), unbiased=False, keepdim=True)
+        y = ((y - m) * torch.rsqrt(v + eps)).reshape(x.shape)
+        y = y * gamma if gamma is not None else y
+        y = y + beta if beta is not None else y
+        return apply_act(y, activation).to(x.dtype)
+    N.dt(x)
+    x = x.contiguous()
+    with on_device(x):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                           for t in (x, gamma, beta)):
+            return _GroupNorm.apply(x, gamma, beta, int(groups), eps, act)
+        return _gn_forward(x, gamma, beta, int(groups), eps, act)[0]
 
 
 # -------------------------------------------------------------- bias + relu
