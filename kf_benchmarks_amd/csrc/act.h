@@ -38,30 +38,50 @@ __device__ __forceinline__ float tanh_f(float u) {
   return copysignf(a < 0.25f ? small : big, u);
 }
 
-// y = act(u).  ``act`` is uniform over a launch: one scalar branch per call.
-__device__ __forceinline__ float act_fwd(float u, int act) {
-  switch (act) {
-    case ACT_RELU: return u > 0.f || u != u ? u : 0.f;  // NaN stays NaN
-    case ACT_RELU6: return u != u ? u : fminf(fmaxf(u, 0.f), 6.f);
-    case ACT_TANH: return tanh_f(u);
-    case ACT_SILU: return siluf(u);
-    default: return u;
+// The piecewise linear ones are y = clamp(u, lo, hi), with comparisons that are
+// false for NaN: NaN stays NaN, and NaN bounds clamp nothing.
+enum ActClass : int { CLAMP = 0, TANH = 1, SILU = 2 };
+
+struct Act {
+  int kind;  // ActClass: a template parameter of the kernels
+  float lo, hi;
+};
+
+inline Act act_of(int code) {
+  const float none = __builtin_nanf("");
+  switch (code) {
+    case ACT_RELU: return Act{CLAMP, 0.f, none};
+    case ACT_RELU6: return Act{CLAMP, 0.f, 6.f};
+    case ACT_TANH: return Act{TANH, none, none};
+    case ACT_SILU: return Act{SILU, none, none};
+    default: return Act{CLAMP, none, none};
   }
 }
 
+template <int KIND> __device__ __forceinline__ float act_fwd(float u, const Act& a) {
+  if constexpr (KIND == TANH) return tanh_f(u);
+  else if constexpr (KIND == SILU) return siluf(u);
+  else return u < a.lo ? a.lo : u > a.hi ? a.hi : u;
+}
+
 // dact/du at u; the gradient at the kinks 0 and 6 is 0.
-__device__ __forceinline__ float act_grad(float u, int act) {
-  switch (act) {
-    case ACT_RELU: return u > 0.f ? 1.f : 0.f;
-    case ACT_RELU6: return u > 0.f && u < 6.f ? 1.f : 0.f;
-    case ACT_TANH: {
-      const float t = tanh_f(u);
-      return 1.f - t * t;
-    }
-    case ACT_SILU: return dsiluf(u);
-    default: return 1.f;
+template <int KIND> __device__ __forceinline__ float act_grad(float u, const Act& a) {
+  if constexpr (KIND == TANH) {
+    const float t = tanh_f(u);
+    return 1.f - t * t;
+  } else if constexpr (KIND == SILU) {
+    return dsiluf(u);
+  } else {
+    return u <= a.lo || u >= a.hi ? 0.f : 1.f;
   }
 }
+
+#define KFB_DISPATCH_ACT(kind, KIND, ...)                             \
+  switch (kind) {                                                     \
+    case kfb::TANH: { constexpr int KIND = kfb::TANH; __VA_ARGS__; break; } \
+    case kfb::SILU: { constexpr int KIND = kfb::SILU; __VA_ARGS__; break; } \
+    default: { constexpr int KIND = kfb::CLAMP; __VA_ARGS__; break; }  \
+  }
 
 // e^v to about 1.5 ulp for any v: the rounding error of log2(e) v, kept from
 // the fused multiply-add, comes back as a first-order factor.

@@ -24,7 +24,8 @@ struct Args {
   void *dx, *dx0;
   const void* dxT;          // gradient of xT or null
   float* part;              // [slabs][K + 1][D], dw | dbias
-  int T, B, D, K, act, reverse;
+  int T, B, D, K, reverse;
+  Act act;
 };
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
@@ -49,7 +50,7 @@ __device__ __forceinline__ void input(const Args& a, int b, int c, int s, int le
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, int KIND>
 __global__ void __launch_bounds__(256) fwd_k(Args a, int runs) {
   const int cv = a.D / V;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -82,14 +83,14 @@ __global__ void __launch_bounds__(256) fwd_k(Args a, int runs) {
         for (int k = 0; k < V; ++k) u[k] = fmaf(a.w[(long)j * a.D + c + k], v[k], u[k]);
       }
 #pragma unroll
-      for (int k = 0; k < V; ++k) u[k] = act_fwd(u[k], a.act);
+      for (int k = 0; k < V; ++k) u[k] = act_fwd<KIND>(u[k], a.act);
     }
     store_vec<T, V>((T*)a.y + row_of(a, b, s, len) * a.D + c, u);
   }
 }
 
 // gradient of u at position s
-template <typename T, int V>
+template <typename T, int V, int KIND>
 __device__ __forceinline__ void pre_grad(const Args& a, int b, int c, int s, int len,
                                          const float (&bias)[V], float (&e)[V]) {
 #pragma unroll
@@ -98,7 +99,7 @@ __device__ __forceinline__ void pre_grad(const Args& a, int b, int c, int s, int
   float u[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) u[k] = bias[k];
-  if (a.act != ACT_LINEAR)
+  if (a.act.kind != CLAMP || a.act.lo == 0.f)
     for (int j = 0; j < a.K; ++j) {
       float v[V];
       input<T, V>(a, b, c, s - a.K + 1 + j, len, v);
@@ -107,12 +108,12 @@ __device__ __forceinline__ void pre_grad(const Args& a, int b, int c, int s, int
     }
   load_vec<T, V>((const T*)a.dy + row_of(a, b, s, len) * a.ldy + c, e);
 #pragma unroll
-  for (int k = 0; k < V; ++k) e[k] *= act_grad(u[k], a.act);
+  for (int k = 0; k < V; ++k) e[k] *= act_grad<KIND>(u[k], a.act);
 }
 
 // dx_s = sum_k w[k] e_{s + K - 1 - k}; for s < 0 that is the state's gradient.
 // The last K - 1 inputs also take the gradient of the state that was returned.
-template <typename T, int V>
+template <typename T, int V, int KIND>
 __global__ void __launch_bounds__(256) dgrad_k(Args a, int runs) {
   const int cv = a.D / V;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(256) dgrad_k(Args a, int runs) {
     if (s < len) {
       for (int j = 0; j < K; ++j) {
         float e[V];
-        pre_grad<T, V>(a, b, c, s + K - 1 - j, len, bias, e);
+        pre_grad<T, V, KIND>(a, b, c, s + K - 1 - j, len, bias, e);
 #pragma unroll
         for (int k = 0; k < V; ++k) g[k] = fmaf(a.w[(long)j * a.D + c + k], e[k], g[k]);
       }
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(256) dgrad_k(Args a, int runs) {
 
 // dw[k] = sum e_s x_{s - K + 1 + k}, dbias = sum e_s: a slab of jobs
 // (sequence, run) per workgroup row, no atomics.
-template <typename T, int V>
+template <typename T, int V, int KIND>
 __global__ void __launch_bounds__(256) wgrad_k(Args a, int runs, int slabs) {
   const int cv = a.D / V;
   const int i = blockIdx.x * 256 + threadIdx.x;
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(256) wgrad_k(Args a, int runs, int slabs) {
     const int b = (int)(job % a.B), s0 = (int)(job / a.B) * RUN, len = seq_len(a, b);
     for (int s = s0; s < min(s0 + RUN, len); ++s) {
       float e[V];
-      pre_grad<T, V>(a, b, c, s, len, bias, e);
+      pre_grad<T, V, KIND>(a, b, c, s, len, bias, e);
 #pragma unroll
       for (int k = 0; k < V; ++k) acc[KMAX][k] += e[k];
 #pragma unroll
@@ -205,7 +206,7 @@ param_grad_k(const float* __restrict__ p, int S, int K, int D, float* dw, float*
 }
 
 // One token: y from the state and x, the state [K-1][B][D] moved on by one.
-template <typename T, int V>
+template <typename T, int V, int KIND>
 __global__ void __launch_bounds__(256) step_k(Args a, T* __restrict__ state) {
   const int cv = a.D / V;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(256) step_k(Args a, T* __restrict__ state) {
     if (j) store_vec<T, V>(state + ((long)(j - 1) * a.B + b) * a.D + c, v);
   }
 #pragma unroll
-  for (int k = 0; k < V; ++k) u[k] = act_fwd(u[k], a.act);
+  for (int k = 0; k < V; ++k) u[k] = act_fwd<KIND>(u[k], a.act);
   store_vec<T, V>((T*)a.y + (long)b * a.D + c, u);
 }
 
@@ -253,15 +254,15 @@ KFB_API hipError_t kfb_cconv_fwd(int dtype, int vec, const void* x, long ldx, co
                                  hipStream_t stream) {
   cconv::Args a{};
   a.x = x; a.ldx = ldx; a.x0 = x0; a.w = w; a.bias = bias; a.len = len; a.y = y; a.xT = xT;
-  a.T = T; a.B = B; a.D = D; a.K = K; a.act = act; a.reverse = reverse;
+  a.T = T; a.B = B; a.D = D; a.K = K; a.act = act_of(act); a.reverse = reverse;
   const int runs = ceil_div(T, cconv::RUN);
   if (cconv::bad(a) || runs > 65534) return hipErrorInvalidValue;
-  KFB_DISPATCH_DTYPE(dtype, E, {
+  KFB_DISPATCH_DTYPE(dtype, E, KFB_DISPATCH_ACT(a.act.kind, KIND, {
     KFB_CCONV_VEC(E, vec, V, {
-      hipLaunchKernelGGL((cconv::fwd_k<E, V>), dim3(ceil_div((long)D / V * B, 256), runs + (xT && K > 1 ? 1 : 0)),
+      hipLaunchKernelGGL((cconv::fwd_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256), runs + (xT && K > 1 ? 1 : 0)),
                          dim3(256), 0, stream, a, runs);
     });
-  });
+  }));
   return hipGetLastError();
 }
 
@@ -273,18 +274,18 @@ KFB_API hipError_t kfb_cconv_bwd(int dtype, int vec, const void* dy, long ldy, c
   cconv::Args a{};
   a.dy = dy; a.ldy = ldy; a.x = x; a.ldx = ldx; a.x0 = x0; a.w = w; a.bias = bias; a.len = len;
   a.dxT = dxT; a.dx = dx; a.dx0 = dx0; a.part = ws;
-  a.T = T; a.B = B; a.D = D; a.K = K; a.act = act; a.reverse = reverse;
+  a.T = T; a.B = B; a.D = D; a.K = K; a.act = act_of(act); a.reverse = reverse;
   const int runs = ceil_div(T, cconv::RUN);
   if (cconv::bad(a) || runs > 65534 || !ws) return hipErrorInvalidValue;
   const int S = cconv::slabs((long)B * runs);
-  KFB_DISPATCH_DTYPE(dtype, E, {
+  KFB_DISPATCH_DTYPE(dtype, E, KFB_DISPATCH_ACT(a.act.kind, KIND, {
     KFB_CCONV_VEC(E, vec, V, {
-      hipLaunchKernelGGL((cconv::dgrad_k<E, V>), dim3(ceil_div((long)D / V * B, 256), runs + (dx0 && K > 1 ? 1 : 0)),
+      hipLaunchKernelGGL((cconv::dgrad_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256), runs + (dx0 && K > 1 ? 1 : 0)),
                          dim3(256), 0, stream, a, runs);
-      hipLaunchKernelGGL((cconv::wgrad_k<E, V>), dim3(ceil_div(D / V, 256), S), dim3(256), 0, stream,
+      hipLaunchKernelGGL((cconv::wgrad_k<E, V, KIND>), dim3(ceil_div(D / V, 256), S), dim3(256), 0, stream,
                          a, runs, S);
     });
-  });
+  }));
   hipLaunchKernelGGL(cconv::param_grad_k, dim3(ceil_div((long)(K + 1) * D, 256)), dim3(256), 0,
                      stream, ws, S, K, D, dw, db, acc_w, acc_b);
   return hipGetLastError();
@@ -295,13 +296,13 @@ KFB_API hipError_t kfb_cconv_step(int dtype, int vec, const void* x, long ldx, v
                                   int act, hipStream_t stream) {
   cconv::Args a{};
   a.x = x; a.ldx = ldx; a.w = w; a.bias = bias; a.y = y;
-  a.T = 1; a.B = B; a.D = D; a.K = K; a.act = act;
+  a.T = 1; a.B = B; a.D = D; a.K = K; a.act = act_of(act);
   if (cconv::bad(a)) return hipErrorInvalidValue;
-  KFB_DISPATCH_DTYPE(dtype, E, {
+  KFB_DISPATCH_DTYPE(dtype, E, KFB_DISPATCH_ACT(a.act.kind, KIND, {
     KFB_CCONV_VEC(E, vec, V, {
-      hipLaunchKernelGGL((cconv::step_k<E, V>), dim3(ceil_div((long)D / V * B, 256)), dim3(256), 0,
+      hipLaunchKernelGGL((cconv::step_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256)), dim3(256), 0,
                          stream, a, (E*)state);
     });
-  });
+  }));
   return hipGetLastError();
 }
