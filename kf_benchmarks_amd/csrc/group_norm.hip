@@ -14,27 +14,14 @@
 //   * split: statistics of row chunks, then an apply pass that merges them in
 //     its prologue (images too large for one workgroup; the second read comes
 //     from the last-level cache while the tensor is below its 256 MB);
+//   * rows (group_norm_rows.hip): one row an image, groups held by lanes;
 //   * gn_*_any_k: one workgroup per group, for groups wider than 512 vectors.
-#include "act.h"
-#include "raw.h"
+#include "group_norm.h"
 
 namespace kfb {
 namespace gn {
 
 constexpr int NT = 256;
-
-struct Args {
-  const void* x;
-  const void* dy;
-  void* y;  // forward: y, backward: dx
-  const float *gamma, *beta;
-  float *mean, *rstd;  // [N][G]
-  float* part;         // backward: [N][2][C], sum e xh | sum e of each image
-  long N, HW;
-  int C, G, cpg;
-  float eps;
-  Act act;
-};
 
 // Sum over the workgroup, the same in every thread.
 __device__ __forceinline__ float block_sum(float v, float* red) {
@@ -187,13 +174,13 @@ __device__ __forceinline__ At place(const Args& a, const Tile& t, long id) {
 
 // tot[image * gb + group] = sum over the rows and the group's channels of the
 // threads' v.  LDS values of a thread: one per vector (fold) or one per channel.
-template <int V>
+template <int V, int VG>
 __device__ __forceinline__ void group_reduce(const Tile& t, const At& p, float* buf, float* tot,
                                              const float (&v)[V]) {
-  const int tid = threadIdx.x, rowlen = t.fold ? t.ncol : t.ncol * V;
+  const int tid = threadIdx.x, rowlen = t.ncol * VG;
   __syncthreads();
   if (p.q < t.sp * t.rp) {
-    if (t.fold) {
+    if constexpr (VG == 1) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < V; ++i) s += v[i];
@@ -221,68 +208,70 @@ __device__ __forceinline__ void group_reduce(const Tile& t, const At& p, float* 
   __syncthreads();
 }
 
-// The value of each of a thread's V channels out of a per-group table.
-template <int V>
-__device__ __forceinline__ void per_channel(const Tile& t, const At& p, const float* tab,
-                                            float (&v)[V]) {
+// The values of a thread's groups out of a table: VG = 1 where every vector lies
+// in one group (fold), else one for each of its V channels.
+template <int V, int VG>
+__device__ __forceinline__ void of_groups(const Tile& t, const At& p, const float* tab,
+                                          float (&v)[VG]) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = p.on ? tab[p.s * t.gb + t.dcpg.div(p.col * V + i)] : 0.f;
+  for (int i = 0; i < VG; ++i) v[i] = p.on ? tab[p.s * t.gb + t.dcpg.div(p.col * V + i)] : 0.f;
 }
 
-template <int V>
-__device__ __forceinline__ void load_params(const float* p, int c, bool on, float other,
-                                            float (&v)[V]) {
+// mean and 1 / std of a thread's groups
+template <int V, int VG>
+__device__ __forceinline__ void load_stats(const Args& a, const Tile& t, const At& p,
+                                           float (&mu)[VG], float (&rs)[VG]) {
+  const int g0 = t.dcpg.div(p.c0);
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = on && p ? p[c + i] : other;
+  for (int i = 0; i < VG; ++i) {
+    const long g = p.n * a.G + g0 + t.dcpg.div(p.col * V + i);
+    mu[i] = p.on ? a.mean[g] : 0.f;
+    rs[i] = p.on ? a.rstd[g] : 0.f;
+  }
 }
 
 // Rows of a chunk in registers (K vectors a thread): mean, then the centred
 // squares, and where the chunk is the image also y.  part: (mean, M2) of the
 // chunks [N][nchunk][G], or null when resident.
-template <typename T, int V, int KIND, int K>
+template <typename T, int V, int VG, int KIND, int K>
 __global__ void __launch_bounds__(512) gn_fwd_tile_k(Args a, Tile t, float2* __restrict__ part) {
   extern __shared__ float lds[];
   float* tot = lds;
   float* buf = lds + t.sp * t.gb;
   for (long id = blockIdx.x; id < t.total; id += gridDim.x) {
     const At p = place<V>(a, t, id);
-    const long rows = min((long)t.rows, a.HW - p.row0);
+    const int rows = p.on ? (int)min((long)t.rows, a.HW - p.row0) : 0;
     const T* __restrict__ x = (const T*)a.x + (p.n * a.HW + p.row0) * a.C + p.c;
     Raw<T, V> raw[K];
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (p.on && p.r + k * t.rp < rows) raw[k].load(x + (long)(p.r + k * t.rp) * a.C);
-    float ga[V], be[V], mu[V], v[V];
-    if (!part) {
-      load_params<V>(a.gamma, p.c, p.on, 1.f, ga);
-      load_params<V>(a.beta, p.c, p.on, 0.f, be);
-    }
+      if (p.r + k * t.rp < rows) raw[k].load(x + (long)(p.r + k * t.rp) * a.C);
+    float mu[VG], v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (p.on && p.r + k * t.rp < rows)
+      if (p.r + k * t.rp < rows)
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] += raw[k][i];
-    const float inv = 1.f / ((float)rows * a.cpg);
-    group_reduce<V>(t, p, buf, tot, v);
-    per_channel<V>(t, p, tot, mu);
-    const float mu_g = threadIdx.x < t.sp * t.gb ? tot[threadIdx.x] * inv : 0.f;
+    const float inv = 1.f / ((float)min((long)t.rows, a.HW - p.row0) * a.cpg);
+    group_reduce<V, VG>(t, p, buf, tot, v);
+    of_groups<V, VG>(t, p, tot, mu);
+    const float mu_g = (int)threadIdx.x < t.sp * t.gb ? tot[threadIdx.x] * inv : 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      mu[i] *= inv;
-      v[i] = 0.f;
-    }
+    for (int i = 0; i < VG; ++i) mu[i] *= inv;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (p.on && p.r + k * t.rp < rows)
+      if (p.r + k * t.rp < rows)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float d = raw[k][i] - mu[i];
+          const float d = raw[k][i] - mu[i % VG];
           v[i] = fmaf(d, d, v[i]);
         }
     // (tot is rewritten behind group_reduce's first barrier)
-    group_reduce<V>(t, p, buf, tot, v);
+    group_reduce<V, VG>(t, p, buf, tot, v);
     if ((int)threadIdx.x < t.sp * t.gb) {
       // thread i: group i % gb of image i / gb (sp gb <= threads, host-checked)
       const int s = t.dgb.div(threadIdx.x), gl = threadIdx.x - s * t.gb;
@@ -298,18 +287,22 @@ __global__ void __launch_bounds__(512) gn_fwd_tile_k(Args a, Tile t, float2* __r
       }
     }
     if (!part) {
-      float sc[V];
-      per_channel<V>(t, p, tot, sc);
+      float sc[V], be[V], m2[VG];
+      load_params<V>(a.gamma, p.c, p.on, 1.f, sc);
+      load_params<V>(a.beta, p.c, p.on, 0.f, be);
+      of_groups<V, VG>(t, p, tot, m2);
       T* __restrict__ y = (T*)a.y + (p.n * a.HW + p.row0) * a.C + p.c;
 #pragma unroll
-      for (int i = 0; i < V; ++i) sc[i] = ga[i] / sqrtf(sc[i] * inv + a.eps);
+      for (int i = 0; i < VG; ++i) m2[i] = 1.f / sqrtf(m2[i] * inv + a.eps);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sc[i] *= m2[i % VG];
 #pragma unroll
       for (int k = 0; k < K; ++k)
-        if (p.on && p.r + k * t.rp < rows) {
+        if (p.r + k * t.rp < rows) {
           float o[V];
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            o[i] = act_fwd<KIND>(fmaf(raw[k][i] - mu[i], sc[i], be[i]), a.act);
+            o[i] = act_fwd<KIND>(fmaf(raw[k][i] - mu[i % VG], sc[i], be[i]), a.act);
           store_vec<T, V>(y + (long)(p.r + k * t.rp) * a.C, o);
         }
     }
@@ -317,9 +310,9 @@ __global__ void __launch_bounds__(512) gn_fwd_tile_k(Args a, Tile t, float2* __r
 }
 
 // Split forward, second pass: the chunks' statistics are merged as
-//   mean = sum n_i mean_i / M,  M2 = sum M2_i + n_i (mean_i - mean)^2,
-// then y for a row chunk (its own chunking).
-template <typename T, int V, int KIND>
+//   mean = sum n_i mean_i / M,  M2 = sum M2_i + n_i (mean_i - mean)^2
+// (16 lanes a group), then y for a row chunk (its own chunking).
+template <typename T, int V, int VG, int KIND>
 __global__ void __launch_bounds__(512)
 gn_apply_k(Args a, Tile t, const float2* __restrict__ part, int pchunk, int prows) {
   extern __shared__ float lds[];
@@ -359,13 +352,13 @@ gn_apply_k(Args a, Tile t, const float2* __restrict__ part, int pchunk, int prow
     }
     __syncthreads();
     if (!p.on) continue;
-    float mu[V], sc[V], ga[V], be[V];
-    per_channel<V>(t, p, mean, mu);
-    per_channel<V>(t, p, rstd, sc);
-    load_params<V>(a.gamma, p.c, true, 1.f, ga);
+    float mu[VG], rs[VG], sc[V], be[V];
+    of_groups<V, VG>(t, p, mean, mu);
+    of_groups<V, VG>(t, p, rstd, rs);
+    load_params<V>(a.gamma, p.c, true, 1.f, sc);
     load_params<V>(a.beta, p.c, true, 0.f, be);
 #pragma unroll
-    for (int i = 0; i < V; ++i) sc[i] *= ga[i];
+    for (int i = 0; i < V; ++i) sc[i] *= rs[i % VG];
     const long base = (p.n * a.HW + p.row0) * a.C + p.c;
     const int rows = (int)min((long)t.rows, a.HW - p.row0);
     const T* __restrict__ x = (const T*)a.x + base;
@@ -382,23 +375,10 @@ gn_apply_k(Args a, Tile t, const float2* __restrict__ part, int pchunk, int prow
           float o[V];
 #pragma unroll
           for (int i = 0; i < V; ++i)
-            o[i] = act_fwd<KIND>(fmaf(raw[k][i] - mu[i], sc[i], be[i]), a.act);
+            o[i] = act_fwd<KIND>(fmaf(raw[k][i] - mu[i % VG], sc[i], be[i]), a.act);
           store_vec<T, V>(y + (long)(r + k * t.rp) * a.C, o);
         }
     }
-  }
-}
-
-// e = dy act'(u) and xh of a thread's V channels
-template <typename T, int V, int KIND>
-__device__ __forceinline__ void grad_terms(const Args& a, const Raw<T, V>& x, const Raw<T, V>& dy,
-                                           const float (&mu)[V], const float (&rs)[V],
-                                           const float (&ga)[V], const float (&be)[V],
-                                           float (&e)[V], float (&xh)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    xh[i] = (x[i] - mu[i]) * rs[i];
-    e[i] = dy[i] * act_grad<KIND>(fmaf(xh[i], ga[i], be[i]), a.act);
   }
 }
 
@@ -421,7 +401,7 @@ __device__ __forceinline__ void channel_reduce(const Tile& t, const At& p, float
 
 // Resident backward: x and dy of whole images in registers.  The channel sums
 // of all tiles of a workgroup go to its slab of part [slabs][2][C].
-template <typename T, int V, int KIND, int K>
+template <typename T, int V, int VG, int KIND, int K>
 __global__ void __launch_bounds__(512) gn_bwd_tile_k(Args a, Tile t) {
   extern __shared__ float lds[];
   float* tot = lds;
@@ -436,30 +416,26 @@ __global__ void __launch_bounds__(512) gn_bwd_tile_k(Args a, Tile t) {
   for (int i = 0; i < V; ++i) cp[i] = cq[i] = 0.f;
   for (long id = blockIdx.x; id < t.total; id += gridDim.x) {
     const At p = place<V>(a, t, id);
+    const int rows = p.on ? (int)a.HW : 0;
     const long base = p.n * a.HW * a.C + p.c;
     const T* __restrict__ x = (const T*)a.x + base;
     const T* __restrict__ dy = (const T*)a.dy + base;
     Raw<T, V> rx[K], rd[K];
-    float mu[V], rs[V], sp[V], sq[V];
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (p.on && p.r + k * t.rp < a.HW) {
+      if (p.r + k * t.rp < rows) {
         rx[k].load(x + (long)(p.r + k * t.rp) * a.C);
         rd[k].load(dy + (long)(p.r + k * t.rp) * a.C);
       }
-    const int g0 = t.dcpg.div(p.c0);
+    float mu[VG], rs[VG], sp[V], sq[V];
+    load_stats<V, VG>(a, t, p, mu, rs);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const long g = p.n * a.G + g0 + t.dcpg.div(p.col * V + i);
-      mu[i] = p.on ? a.mean[g] : 0.f;
-      rs[i] = p.on ? a.rstd[g] : 0.f;
-      sp[i] = sq[i] = 0.f;
-    }
+    for (int i = 0; i < V; ++i) sp[i] = sq[i] = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (p.on && p.r + k * t.rp < a.HW) {
+      if (p.r + k * t.rp < rows) {
         float e[V], xh[V];
-        grad_terms<T, V, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
+        grad_terms<T, V, VG, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           sp[i] += e[i];
@@ -473,19 +449,20 @@ __global__ void __launch_bounds__(512) gn_bwd_tile_k(Args a, Tile t) {
       sp[i] *= ga[i];
       sq[i] *= ga[i];
     }
-    group_reduce<V>(t, p, buf, tot, sp);
-    group_reduce<V>(t, p, buf, tot2, sq);
-    per_channel<V>(t, p, tot, sp);
-    per_channel<V>(t, p, tot2, sq);
+    group_reduce<V, VG>(t, p, buf, tot, sp);
+    group_reduce<V, VG>(t, p, buf, tot2, sq);
+    float s1[VG], s2[VG];
+    of_groups<V, VG>(t, p, tot, s1);
+    of_groups<V, VG>(t, p, tot2, s2);
     T* __restrict__ dx = (T*)a.y + base;
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      if (p.on && p.r + k * t.rp < a.HW) {
+      if (p.r + k * t.rp < rows) {
         float e[V], xh[V];
-        grad_terms<T, V, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
+        grad_terms<T, V, VG, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          e[i] = rs[i] * (fmaf(ga[i], e[i], -sp[i] * inv) - xh[i] * (sq[i] * inv));
+          e[i] = rs[i % VG] * (fmaf(ga[i], e[i], -s1[i % VG] * inv) - xh[i] * (s2[i % VG] * inv));
         store_vec<T, V>(dx + (long)(p.r + k * t.rp) * a.C, e);
       }
   }
@@ -494,24 +471,20 @@ __global__ void __launch_bounds__(512) gn_bwd_tile_k(Args a, Tile t) {
   channel_reduce<V>(t, p0, buf, cp, out + a.C);
 }
 
-// Split backward, first pass: channel sums of a row chunk into
-// part [N * nchunk][2][C].
-template <typename T, int V, int KIND>
-__global__ void __launch_bounds__(512) gn_bwd_sums_k(Args a, Tile t) {
+// Split backward, first pass: a row chunk's channel sums into part
+// [N * nchunk][2][C] and its (s1, s2) into gpart [N * nchunk][G].
+template <typename T, int V, int VG, int KIND>
+__global__ void __launch_bounds__(512) gn_bwd_sums_k(Args a, Tile t, float2* __restrict__ gpart) {
   extern __shared__ float lds[];
+  float *tot = lds, *tot2 = lds + t.gb, *buf = lds + 2 * t.gb;
   for (long id = blockIdx.x; id < t.total; id += gridDim.x) {
     const At p = place<V>(a, t, id);
-    float sp[V], sq[V], mu[V], rs[V], ga[V], be[V];
+    float sp[V], sq[V], mu[VG], rs[VG], ga[V], be[V];
     load_params<V>(a.gamma, p.c, p.on, 1.f, ga);
     load_params<V>(a.beta, p.c, p.on, 0.f, be);
-    const int g0 = t.dcpg.div(p.c0);
+    load_stats<V, VG>(a, t, p, mu, rs);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const long g = p.n * a.G + g0 + t.dcpg.div(p.col * V + i);
-      mu[i] = p.on ? a.mean[g] : 0.f;
-      rs[i] = p.on ? a.rstd[g] : 0.f;
-      sp[i] = sq[i] = 0.f;
-    }
+    for (int i = 0; i < V; ++i) sp[i] = sq[i] = 0.f;
     const long base = (p.n * a.HW + p.row0) * a.C + p.c;
     const int rows = p.on ? (int)min((long)t.rows, a.HW - p.row0) : 0;
     const T* __restrict__ x = (const T*)a.x + base;
@@ -529,7 +502,7 @@ __global__ void __launch_bounds__(512) gn_bwd_sums_k(Args a, Tile t) {
       for (int k = 0; k < U; ++k)
         if (r + k * t.rp < rows) {
           float e[V], xh[V];
-          grad_terms<T, V, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
+          grad_terms<T, V, VG, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
 #pragma unroll
           for (int i = 0; i < V; ++i) {
             sp[i] += e[i];
@@ -537,43 +510,84 @@ __global__ void __launch_bounds__(512) gn_bwd_sums_k(Args a, Tile t) {
           }
         }
     }
-    float* out = a.part + id / t.nblk * 2 * a.C + p.c0;
-    channel_reduce<V>(t, p, lds, sq, out);
-    channel_reduce<V>(t, p, lds, sp, out + a.C);
+    const long slab = id / t.nblk;
+    float* out = a.part + slab * 2 * a.C + p.c0;
+    channel_reduce<V>(t, p, buf, sq, out);
+    channel_reduce<V>(t, p, buf, sp, out + a.C);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      sp[i] *= ga[i];
+      sq[i] *= ga[i];
+    }
+    group_reduce<V, VG>(t, p, buf, tot, sp);
+    group_reduce<V, VG>(t, p, buf, tot2, sq);
+    if ((int)threadIdx.x < p.gbw)
+      gpart[slab * a.G + t.dcpg.div(p.c0) + threadIdx.x] = make_float2(tot[threadIdx.x], tot2[threadIdx.x]);
   }
 }
 
-// Split backward, second pass: s1 and s2 of the groups from the channel sums,
-// then dx.
-template <typename T, int V, int KIND>
-__global__ void __launch_bounds__(512) gn_bwd_apply_k(Args a, Tile t, int pchunk) {
+// dgamma / dbeta = sum over the slabs of part [S][2][C], in a fixed order: the
+// same sum on every run.  16 of the 2 C columns x blockDim / 16 rows a workgroup.
+struct ParamGrad {
+  const float* part;
+  float *dgamma, *dbeta;
+  long S;
+  int C, acc_g, acc_b, blocks;
+};
+
+__device__ __forceinline__ void param_grad(const ParamGrad& q, int block, float* red) {
+  const int nt = blockDim.x, cl = threadIdx.x % 16, r0 = threadIdx.x / 16, nr = nt / 16;
+  const int c = block * 16 + cl;
+  constexpr int U = 8;
+  float s[U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) s[k] = 0.f;
+  if (c < 2 * q.C)
+    for (long r = r0; r < q.S; r += U * nr)
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (r + nr * k < q.S) s[k] += q.part[(r + nr * k) * 2 * q.C + c];
+  red[threadIdx.x] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  __syncthreads();
+  if (r0 == 0 && c < 2 * q.C) {
+    float sum = 0.f;
+    for (int r = 0; r < nr; ++r) sum += red[r * 16 + cl];
+    float* out = c < q.C ? q.dgamma : q.dbeta;
+    const int acc = c < q.C ? q.acc_g : q.acc_b, i = c < q.C ? c : c - q.C;
+    if (out) out[i] = acc ? out[i] + sum : sum;
+  }
+}
+
+__global__ void __launch_bounds__(1024) gn_param_grad_k(ParamGrad q) {
+  __shared__ float red[1024];
+  param_grad(q, blockIdx.x, red);
+}
+
+// Split backward, second pass: the first q.blocks workgroups sum dgamma and
+// dbeta; the others merge (s1, s2) of their groups and write dx.
+template <typename T, int V, int VG, int KIND>
+__global__ void __launch_bounds__(512)
+gn_bwd_apply_k(Args a, Tile t, const float2* __restrict__ gpart, int pchunk, ParamGrad q) {
   extern __shared__ float lds[];
-  float *s1 = lds, *s2 = lds + t.gb, *cs = lds + 2 * t.gb;  // cs [2][cb]
+  if ((int)blockIdx.x < q.blocks) {
+    param_grad(q, blockIdx.x, lds);
+    return;
+  }
+  float *s1 = lds, *s2 = lds + t.gb;
   const float inv = 1.f / ((float)a.HW * a.cpg);
-  for (long id = blockIdx.x; id < t.total; id += gridDim.x) {
+  for (long id = blockIdx.x - q.blocks; id < t.total; id += gridDim.x - q.blocks) {
     const At p = place<V>(a, t, id);
     const long n = id / t.nblk / t.nchunk;
     const int g0 = t.dcpg.div(p.c0);
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.cbw; c += t.nt) {
-      const float* q = a.part + n * pchunk * 2 * a.C + p.c0 + c;
-      float u = 0.f, v = 0.f;
-      for (int i = 0; i < pchunk; ++i) {
-        v += q[(long)i * 2 * a.C];
-        u += q[(long)i * 2 * a.C + a.C];
-      }
-      const float ga = a.gamma ? a.gamma[p.c0 + c] : 1.f;
-      cs[c] = ga * u;
-      cs[t.cb + c] = ga * v;
-    }
     __syncthreads();
     const int j = threadIdx.x & 15;
     for (int gl = threadIdx.x >> 4; gl < t.gb; gl += t.nt >> 4) {
       float u = 0.f, v = 0.f;
       if (gl < p.gbw)
-        for (int c = j; c < a.cpg; c += 16) {
-          u += cs[gl * a.cpg + c];
-          v += cs[t.cb + gl * a.cpg + c];
+        for (int i = j; i < pchunk; i += 16) {
+          const float2 w = gpart[(n * pchunk + i) * a.G + g0 + gl];
+          u += w.x;
+          v += w.y;
         }
       for (int o = 8; o > 0; o >>= 1) {
         u += __shfl_xor(u, o, 64);
@@ -586,17 +600,12 @@ __global__ void __launch_bounds__(512) gn_bwd_apply_k(Args a, Tile t, int pchunk
     }
     __syncthreads();
     if (!p.on) continue;
-    float sp[V], sq[V], mu[V], rs[V], ga[V], be[V];
-    per_channel<V>(t, p, s1, sp);
-    per_channel<V>(t, p, s2, sq);
+    float sp[VG], sq[VG], mu[VG], rs[VG], ga[V], be[V];
+    of_groups<V, VG>(t, p, s1, sp);
+    of_groups<V, VG>(t, p, s2, sq);
     load_params<V>(a.gamma, p.c, true, 1.f, ga);
     load_params<V>(a.beta, p.c, true, 0.f, be);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const long g = p.n * a.G + g0 + t.dcpg.div(p.col * V + i);
-      mu[i] = a.mean[g];
-      rs[i] = a.rstd[g];
-    }
+    load_stats<V, VG>(a, t, p, mu, rs);
     const long base = (p.n * a.HW + p.row0) * a.C + p.c;
     const int rows = (int)min((long)t.rows, a.HW - p.row0);
     const T* __restrict__ x = (const T*)a.x + base;
@@ -615,37 +624,13 @@ __global__ void __launch_bounds__(512) gn_bwd_apply_k(Args a, Tile t, int pchunk
       for (int k = 0; k < U; ++k)
         if (r + k * t.rp < rows) {
           float e[V], xh[V];
-          grad_terms<T, V, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
+          grad_terms<T, V, VG, KIND>(a, rx[k], rd[k], mu, rs, ga, be, e, xh);
 #pragma unroll
-          for (int i = 0; i < V; ++i) e[i] = rs[i] * (fmaf(ga[i], e[i], -sp[i]) - xh[i] * sq[i]);
+          for (int i = 0; i < V; ++i)
+            e[i] = rs[i % VG] * (fmaf(ga[i], e[i], -sp[i % VG]) - xh[i] * sq[i % VG]);
           store_vec<T, V>(dx + (long)(r + k * t.rp) * a.C, e);
         }
     }
-  }
-}
-
-// dgamma / dbeta = sum over the slabs of part [S][2][C], in a fixed order: the
-// same sum on every run.  16 columns x 64 rows a workgroup.
-__global__ void __launch_bounds__(1024)
-gn_param_grad_k(const float* __restrict__ part, long S, int C, float* __restrict__ dgamma,
-                float* __restrict__ dbeta, int acc_g, int acc_b) {
-  __shared__ float red[16][65];
-  const int cl = threadIdx.x % 16, r0 = threadIdx.x / 16;
-  const int c = blockIdx.x * 16 + cl;  // of 2 C
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < 2 * C)
-    for (long r = r0; r < S; r += 256)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (r + 64 * k < S) s[k] += part[(r + 64 * k) * 2 * C + c];
-  red[cl][r0] = (s[0] + s[1]) + (s[2] + s[3]);
-  __syncthreads();
-  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, cc = blockIdx.x * 16 + w;
-  const float sum = wave_sum(red[w][lane]);
-  if (lane == 0 && cc < 2 * C) {
-    float* out = cc < C ? dgamma : dbeta;
-    const int acc = cc < C ? acc_g : acc_b, i = cc < C ? cc : cc - C;
-    if (out) out[i] = acc ? out[i] + sum : sum;
   }
 }
 
@@ -653,14 +638,14 @@ gn_param_grad_k(const float* __restrict__ part, long S, int C, float* __restrict
 // most vectors a thread holds (forward: x, backward: x and dy each), most threads
 constexpr int KF = 16, KB = 8, NTMAX = 512;
 
-enum How : int { ANY, RESIDENT, SPLIT };
+enum How : int { ANY, RESIDENT, SPLIT, ROWS };
 
 struct Plan {
   How how;
   int V, K;
   Tile t;       // resident, or the statistics pass of the split
   Tile apply;   // split: the apply pass
-  int grid_y_slabs;
+  int slabs;    // resident backward: slabs of channel sums
   long ws;      // floats
 };
 
@@ -700,6 +685,11 @@ inline Plan plan(int dtype, long N, long HW, int C, int G, int V, bool bwd) {
   p.V = V;
   p.how = ANY;
   p.ws = bwd ? N * 2 * C : 0;
+  if (rows_take(dtype, N, HW, C, G, V)) {
+    p.how = ROWS;
+    p.ws = bwd ? rows_slabs(dtype, N, C, G, V) * 2 * C : 0;
+    return p;
+  }
   Tile& t = p.t;
   t.cb = column_block(C, cpg, V, esz, 128);
   t.ncol = t.cb / V;
@@ -729,8 +719,8 @@ inline Plan plan(int dtype, long N, long HW, int C, int G, int V, bool bwd) {
     // a slab of channel sums per workgroup row: enough workgroups to fill the card
     const long per = t.total / t.nblk;
     const long most = ceil_div(2048, t.nblk);
-    p.grid_y_slabs = (int)(per < most ? per : most);
-    p.ws = bwd ? (long)p.grid_y_slabs * 2 * C : 0;
+    p.slabs = (int)(per < most ? per : most);
+    p.ws = bwd ? (long)p.slabs * 2 * C : 0;
     return p;
   }
   // split
@@ -745,7 +735,10 @@ inline Plan plan(int dtype, long N, long HW, int C, int G, int V, bool bwd) {
   p.how = SPLIT;
   p.apply = t;
   p.K = 16;
-  const long want = 2048;
+  // workgroups that fill the card: fewer mean longer chunks and fewer partial
+  // sums to merge (2048 of them took 41 us in the forward's second pass and 73
+  // in the backward's at 32 x 56 x 56 x 256, 1024: see the table below)
+  const long want = 1024;
   // forward statistics: chunks that fit the registers
   while (!bwd && p.K > 4 && N * t.nblk * ceil_div(HW, (long)t.rp * p.K) < want) p.K /= 2;
   long chunks = ceil_div(want, N * t.nblk);
@@ -758,7 +751,7 @@ inline Plan plan(int dtype, long N, long HW, int C, int G, int V, bool bwd) {
   };
   set(t, bwd ? ceil_div(HW, chunks) : (long)t.rp * p.K);
   set(p.apply, ceil_div(HW, chunks));
-  p.ws = bwd ? N * t.nchunk * 2 * C : N * t.nchunk * G * 2;
+  p.ws = bwd ? N * t.nchunk * (2 * C + 2 * G) : N * t.nchunk * G * 2;
   return p;
 }
 
@@ -797,10 +790,16 @@ inline int vec(int dtype, int C, const void* p, const void* q, const void* r) {
 }  // namespace gn
 }  // namespace kfb
 
-#define KFB_GN_VEC(T, v, V, ...)                                             \
-  if (v > 2) { constexpr int V = 16 / sizeof(T); __VA_ARGS__; }                \
-  else if (v == 2 && sizeof(T) == 2) { constexpr int V = 2; __VA_ARGS__; }     \
-  else { constexpr int V = 1; __VA_ARGS__; }
+#define KFB_GN_VEC(T, v, fold, V, VG, ...)                                            \
+  if (v > 2) {                                                                        \
+    constexpr int V = 16 / sizeof(T);                                                 \
+    if (fold) { constexpr int VG = 1; __VA_ARGS__; }                                   \
+    else { constexpr int VG = V; __VA_ARGS__; }                                        \
+  } else if (v == 2 && sizeof(T) == 2) {                                              \
+    constexpr int V = 2;                                                              \
+    if (fold) { constexpr int VG = 1; __VA_ARGS__; }                                   \
+    else { constexpr int VG = V; __VA_ARGS__; }                                        \
+  } else { constexpr int V = 1, VG = 1; __VA_ARGS__; }
 
 #define KFB_GN_K(k, K, ...)                               \
   switch (k) {                                            \
@@ -838,22 +837,23 @@ KFB_API hipError_t kfb_gn_fwd(int dtype, const void* x, void* y, long N, long HW
   if (gn::bad(N, HW, C, G)) return hipErrorInvalidValue;
   gn::Args a{x, nullptr, y, gamma, beta, mean, rstd, nullptr, N, HW, C, G, C / G, eps, act_of(act)};
   const gn::Plan p = gn::plan(dtype, N, HW, C, G, gn::vec(dtype, C, x, y, nullptr), false);
+  if (p.how == gn::ROWS) return gn::rows_fwd(dtype, a, p.V, stream);
   KFB_DISPATCH_DTYPE(dtype, T, KFB_DISPATCH_ACT(a.act.kind, KIND, {
     if (p.how == gn::ANY) {
       hipLaunchKernelGGL((gn::gn_fwd_any_k<T, KIND>), gn::groups_grid(N, G), dim3(gn::NT), 0, stream, a,
                          gn::columns(C / G));
     } else {
-      KFB_GN_VEC(T, p.V, V, {
-        const size_t shm = sizeof(float) * ((size_t)p.t.sp * p.t.gb + (size_t)p.t.nt * (p.t.fold ? 1 : V));
+      KFB_GN_VEC(T, p.V, p.t.fold, V, VG, {
+        const size_t shm = sizeof(float) * ((size_t)p.t.sp * p.t.gb + (size_t)p.t.nt * VG);
         float2* part = p.how == gn::SPLIT ? (float2*)ws : nullptr;
         KFB_GN_K(p.K, K, {
-          hipLaunchKernelGGL((gn::gn_fwd_tile_k<T, V, KIND, K>), gn::tiles_grid(p.t), dim3(p.t.nt), shm,
-                             stream, a, p.t, part);
+          hipLaunchKernelGGL((gn::gn_fwd_tile_k<T, V, VG, KIND, K>), gn::tiles_grid(p.t),
+                             dim3(p.t.nt), shm, stream, a, p.t, part);
         });
         if (part)
-          hipLaunchKernelGGL((gn::gn_apply_k<T, V, KIND>), gn::tiles_grid(p.apply), dim3(p.apply.nt),
-                             2 * sizeof(float) * p.apply.gb, stream, a, p.apply, part, p.t.nchunk,
-                             p.t.rows);
+          hipLaunchKernelGGL((gn::gn_apply_k<T, V, VG, KIND>), gn::tiles_grid(p.apply),
+                             dim3(p.apply.nt), 2 * sizeof(float) * p.apply.gb, stream, a, p.apply,
+                             part, p.t.nchunk, p.t.rows);
       });
     }
   }));
@@ -867,35 +867,47 @@ KFB_API hipError_t kfb_gn_bwd(int dtype, const void* dy, const void* x, void* dx
   if (gn::bad(N, HW, C, G) || !ws) return hipErrorInvalidValue;
   gn::Args a{x, dy, dx, gamma, beta, (float*)mean, (float*)rstd, ws, N, HW, C, G, C / G, 0.f, act_of(act)};
   const gn::Plan p = gn::plan(dtype, N, HW, C, G, gn::vec(dtype, C, x, dy, dx), true);
-  long slabs = N;
+  gn::ParamGrad q{ws, dgamma, dbeta, N, C, acc_gamma, acc_beta, ceil_div(2 * C, 16)};
+  const bool params = dgamma || dbeta;
+  bool done = false;
+  if (p.how == gn::ROWS) {
+    q.S = gn::rows_slabs(dtype, N, C, G, p.V);
+    const hipError_t err = gn::rows_bwd(dtype, a, p.V, stream);
+    if (err != hipSuccess) return err;
+  } else
   KFB_DISPATCH_DTYPE(dtype, T, KFB_DISPATCH_ACT(a.act.kind, KIND, {
     if (p.how == gn::ANY) {
-      hipLaunchKernelGGL((gn::gn_bwd_any_k<T, KIND>), gn::groups_grid(N, G), dim3(gn::NT), 0, stream, a,
-                         gn::columns(C / G));
+      hipLaunchKernelGGL((gn::gn_bwd_any_k<T, KIND>), gn::groups_grid(N, G), dim3(gn::NT), 0, stream,
+                         a, gn::columns(C / G));
     } else {
-      KFB_GN_VEC(T, p.V, V, {
-        const size_t buf = sizeof(float) * (size_t)p.t.nt * V;
+      KFB_GN_VEC(T, p.V, p.t.fold, V, VG, {
+        const size_t buf = sizeof(float) * ((size_t)p.t.nt * V + 2 * (size_t)p.t.sp * p.t.gb);
         if (p.how == gn::RESIDENT) {
-          slabs = p.grid_y_slabs;
-          const size_t shm = buf + 2 * sizeof(float) * (size_t)p.t.sp * p.t.gb;
+          q.S = p.slabs;
           KFB_GN_K(p.K, K, {
             if constexpr (K <= gn::KB)
-              hipLaunchKernelGGL((gn::gn_bwd_tile_k<T, V, KIND, K>),
-                                 dim3((unsigned)(slabs * p.t.nblk)), dim3(p.t.nt), shm, stream, a, p.t);
+              hipLaunchKernelGGL((gn::gn_bwd_tile_k<T, V, VG, KIND, K>),
+                                 dim3((unsigned)(p.slabs * p.t.nblk)), dim3(p.t.nt), buf, stream, a,
+                                 p.t);
           });
         } else {
-          slabs = N * p.t.nchunk;
-          hipLaunchKernelGGL((gn::gn_bwd_sums_k<T, V, KIND>), gn::tiles_grid(p.t), dim3(p.t.nt), buf, stream,
-                             a, p.t);
-          hipLaunchKernelGGL((gn::gn_bwd_apply_k<T, V, KIND>), gn::tiles_grid(p.apply), dim3(p.apply.nt),
-                             2 * sizeof(float) * (size_t)(p.apply.gb + p.apply.cb), stream, a, p.apply,
-                             p.t.nchunk);
+          q.S = N * p.t.nchunk;
+          float2* gpart = (float2*)(ws + q.S * 2 * C);
+          hipLaunchKernelGGL((gn::gn_bwd_sums_k<T, V, VG, KIND>), gn::tiles_grid(p.t), dim3(p.t.nt),
+                             buf, stream, a, p.t, gpart);
+          if (!params) q.blocks = 0;
+          dim3 grid = gn::tiles_grid(p.apply);
+          grid.x += q.blocks;
+          size_t shm = 2 * sizeof(float) * (size_t)p.apply.gb;
+          if (shm < sizeof(float) * p.apply.nt) shm = sizeof(float) * p.apply.nt;
+          hipLaunchKernelGGL((gn::gn_bwd_apply_k<T, V, VG, KIND>), grid, dim3(p.apply.nt), shm, stream,
+                             a, p.apply, gpart, p.t.nchunk, q);
+          done = true;
         }
       });
     }
   }));
-  if (dgamma || dbeta)
-    hipLaunchKernelGGL(gn::gn_param_grad_k, dim3(ceil_div(2 * C, 16)), dim3(1024), 0, stream, ws,
-                       slabs, C, dgamma, dbeta, acc_gamma, acc_beta);
+  if (params && !done)
+    hipLaunchKernelGGL(gn::gn_param_grad_k, dim3(q.blocks), dim3(1024), 0, stream, q);
   return hipGetLastError();
 }
