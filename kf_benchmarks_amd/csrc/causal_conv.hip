@@ -5,15 +5,18 @@
 // or zero.  Position s is time s, or len - 1 - s in reverse; rows at or past a
 // sequence's length give y = 0 and take no gradient.
 //
-// Bound by HBM.  A thread owns V channels (16 bytes) of one sequence and a run
-// of RUN positions, with the last K inputs in registers: each input is read
-// once, and the K - 1 inputs before a run once more (from cache).
+// Bound by HBM.  A thread owns V channels of one sequence and a run of positions,
+// with the last K inputs (backward: also the last K gradients of u) in registers
+// and U loads in flight: each input is read once, and the K - 1 rows next to a
+// run once more (from cache).  u is computed again in the backward, nothing but x
+// is kept.
 #include "act.h"
+#include "raw.h"
 
 namespace kfb {
 namespace cconv {
 
-constexpr int RUN = 16, KMAX = 8;
+constexpr int KMAX = 8, U = 8;  // most taps; positions whose loads are in flight together
 
 struct Args {
   const void *x, *dy, *x0;  // x0: state [K-1][B][D] or null
@@ -32,177 +35,251 @@ __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.T) : a.T;
 }
 
-__device__ __forceinline__ long row_of(const Args& a, int b, int s, int len) {
-  const int t = a.reverse && s < len ? len - 1 - s : s;
-  return (long)t * a.B + b;
-}
+// One sequence's rows of a [T][B] tensor: position s (< len) at base + s * step.
+template <typename T> struct Line {
+  T* base;
+  long step;
+};
 
-// input at position s (< len) of sequence b: the state for s < 0
-template <typename T, int V>
-__device__ __forceinline__ void input(const Args& a, int b, int c, int s, int len, float (&v)[V]) {
-  if (s >= 0 && s < len) {
-    load_vec<T, V>((const T*)a.x + row_of(a, b, s, len) * a.ldx + c, v);
-  } else if (s < 0 && s >= 1 - a.K && a.x0) {
-    load_vec<T, V>((const T*)a.x0 + ((long)(s + a.K - 1) * a.B + b) * a.D + c, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
+template <typename T>
+__device__ __forceinline__ Line<T> line(const Args& a, T* p, long ld, int b, int c, int len) {
+  const long step = (long)a.B * ld;
+  Line<T> l{p + (long)b * ld + c, step};
+  if (a.reverse && len > 0) {
+    l.base += (len - 1) * step;
+    l.step = -step;
   }
+  return l;
 }
 
-template <typename T, int V, int KIND>
-__global__ void __launch_bounds__(256) fwd_k(Args a, int runs) {
+// the input at position s < len: the state for s < 0
+template <typename T, int V>
+__device__ __forceinline__ void input(const Args& a, const Line<const T>& x, int b, int c, int s,
+                                      int len, Raw<T, V>& v) {
+  if (s >= 0 && s < len) v.load(x.base + s * x.step);
+  else if (s < 0 && s >= 1 - a.K && a.x0) v.load((const T*)a.x0 + ((long)(s + a.K - 1) * a.B + b) * a.D + c);
+  else v.zero();
+}
+
+// w[j], j = 0..KP-1, are the taps of the inputs s - KP + 1 .. s; those before the
+// K used ones are skipped, not multiplied by zero (0 * inf).
+template <int KP, int V>
+__device__ __forceinline__ void load_taps(const Args& a, int c, float (&w)[KP][V]) {
+#pragma unroll
+  for (int j = 0; j < KP; ++j)
+#pragma unroll
+    for (int k = 0; k < V; ++k) w[j][k] = j >= KP - a.K ? a.w[(long)(j - KP + a.K) * a.D + c + k] : 0.f;
+}
+
+template <typename T, int V, int KIND, int KP, bool EXACT>
+__global__ void __launch_bounds__(256) fwd_k(Args a, int run, int runs) {
   const int cv = a.D / V;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= (long)cv * a.B) return;
-  const int c = (int)(i % cv) * V, b = (int)(i / cv), K = a.K;
+  const int c = (int)(i % cv) * V, b = (int)(i / cv), skip = EXACT ? 0 : KP - a.K;
   const int len = seq_len(a, b);
+  const Line<const T> x = line(a, (const T*)a.x, a.ldx, b, c, len);
   if ((int)blockIdx.y == runs) {  // the state after the last position
-    for (int j = 0; j < K - 1; ++j) {
-      float v[V];
-      input<T, V>(a, b, c, len - (K - 1) + j, len, v);
-      store_vec<T, V>((T*)a.xT + ((long)j * a.B + b) * a.D + c, v);
+    for (int j = 0; j < a.K - 1; ++j) {
+      Raw<T, V> v;
+      float f[V];
+      input<T, V>(a, x, b, c, len - (a.K - 1) + j, len, v);
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] = v[k];
+      store_vec<T, V>((T*)a.xT + ((long)j * a.B + b) * a.D + c, f);
     }
     return;
   }
-  float bias[V];
+  const Line<T> y = line(a, (T*)a.y, (long)a.D, b, c, len);
+  float w[KP][V], bias[V];
+  load_taps<KP, V>(a, c, w);
 #pragma unroll
   for (int k = 0; k < V; ++k) bias[k] = a.bias ? a.bias[c + k] : 0.f;
-  const int s0 = blockIdx.y * RUN, s1 = min(s0 + RUN, a.T);
-  for (int s = s0; s < s1; ++s) {
-    float u[V];
+  const int s0 = blockIdx.y * run, s1 = min(s0 + run, a.T);
+  Raw<T, V> win[KP - 1 + U];
 #pragma unroll
-    for (int k = 0; k < V; ++k) u[k] = 0.f;
-    if (s < len) {
+  for (int j = 0; j < KP - 1; ++j) input<T, V>(a, x, b, c, s0 - KP + 1 + j, len, win[j]);
+  for (int s = s0; s < s1; s += U) {
+#pragma unroll
+    for (int r = 0; r < U; ++r) input<T, V>(a, x, b, c, s + r, len, win[KP - 1 + r]);
+#pragma unroll
+    for (int r = 0; r < U; ++r) {
+      if (s + r >= s1) break;
+      float u[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) u[k] = bias[k];
-      for (int j = 0; j < K; ++j) {
-        float v[V];
-        input<T, V>(a, b, c, s - K + 1 + j, len, v);
 #pragma unroll
-        for (int k = 0; k < V; ++k) u[k] = fmaf(a.w[(long)j * a.D + c + k], v[k], u[k]);
-      }
+      for (int j = 0; j < KP; ++j)
+        if (EXACT || j >= skip)
 #pragma unroll
-      for (int k = 0; k < V; ++k) u[k] = act_fwd<KIND>(u[k], a.act);
+          for (int k = 0; k < V; ++k) u[k] = fmaf(w[j][k], win[r + j][k], u[k]);
+#pragma unroll
+      for (int k = 0; k < V; ++k) u[k] = s + r < len ? act_fwd<KIND>(u[k], a.act) : 0.f;
+      T* at = s + r < len ? y.base + (s + r) * y.step : (T*)a.y + ((long)(s + r) * a.B + b) * a.D + c;
+      store_vec<T, V>(at, u);
     }
-    store_vec<T, V>((T*)a.y + row_of(a, b, s, len) * a.D + c, u);
+#pragma unroll
+    for (int j = 0; j < KP - 1; ++j) win[j] = win[U + j];
   }
 }
 
-// gradient of u at position s
-template <typename T, int V, int KIND>
-__device__ __forceinline__ void pre_grad(const Args& a, int b, int c, int s, int len,
-                                         const float (&bias)[V], float (&e)[V]) {
+// Going up through the positions p of a run and the K - 1 behind it:
+//   e_p = dy_p act'(u_p);  dw[k] += e_p x_{p-K+1+k}, dbias += e_p (p in the run);
+//   dx_s = sum_k w[k] e_{s+K-1-k} is complete at p = s + K - 1; s < 0 is the state,
+//   and the last K - 1 inputs take the gradient of the state that was returned.
+// A workgroup is CX column vectors x 256 / CX jobs (sequence, run); its parameter
+// sums go to its slab of part, no atomics.
+template <typename T, int V, int KIND, int KP, bool EXACT, int CX>
+__global__ void __launch_bounds__(256) bwd_k(Args a, int run, int runs) {
+  constexpr int JY = 256 / CX;
+  __shared__ float red[JY][CX * V + 1];
+  const int K = EXACT ? KP : a.K, skip = KP - K;
+  const int cl = threadIdx.x % CX, ty = threadIdx.x / CX;
+  const int c = (blockIdx.x * CX + cl) * V;
+  const bool on = c < a.D;
+  float w[KP][V], bias[V], dw[KP][V], db[V];
 #pragma unroll
-  for (int k = 0; k < V; ++k) e[k] = 0.f;
-  if (s < 0 || s >= len) return;
-  float u[V];
+  for (int j = 0; j < KP; ++j)
 #pragma unroll
-  for (int k = 0; k < V; ++k) u[k] = bias[k];
-  if (a.act.kind != CLAMP || a.act.lo == 0.f)
-    for (int j = 0; j < a.K; ++j) {
-      float v[V];
-      input<T, V>(a, b, c, s - a.K + 1 + j, len, v);
+    for (int k = 0; k < V; ++k) dw[j][k] = w[j][k] = 0.f;
 #pragma unroll
-      for (int k = 0; k < V; ++k) u[k] = fmaf(a.w[(long)j * a.D + c + k], v[k], u[k]);
-    }
-  load_vec<T, V>((const T*)a.dy + row_of(a, b, s, len) * a.ldy + c, e);
+  for (int k = 0; k < V; ++k) db[k] = bias[k] = 0.f;
+  float wl[EXACT ? 1 : KP][V];  // tap j at j, where w has it at j + skip
+  if constexpr (!EXACT)
 #pragma unroll
-  for (int k = 0; k < V; ++k) e[k] *= act_grad<KIND>(u[k], a.act);
-}
-
-// dx_s = sum_k w[k] e_{s + K - 1 - k}; for s < 0 that is the state's gradient.
-// The last K - 1 inputs also take the gradient of the state that was returned.
-template <typename T, int V, int KIND>
-__global__ void __launch_bounds__(256) dgrad_k(Args a, int runs) {
-  const int cv = a.D / V;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long)cv * a.B) return;
-  const int c = (int)(i % cv) * V, b = (int)(i / cv), K = a.K;
-  const int len = seq_len(a, b);
-  float bias[V];
+    for (int j = 0; j < KP; ++j)
 #pragma unroll
-  for (int k = 0; k < V; ++k) bias[k] = a.bias ? a.bias[c + k] : 0.f;
-  const bool state = (int)blockIdx.y == runs;
-  const int s0 = state ? 1 - K : blockIdx.y * RUN, s1 = state ? 0 : min(s0 + RUN, a.T);
-  for (int s = s0; s < s1; ++s) {
-    float g[V];
+      for (int k = 0; k < V; ++k) wl[j][k] = on && j < K ? a.w[(long)j * a.D + c + k] : 0.f;
+  if (on) {
+    load_taps<KP, V>(a, c, w);
 #pragma unroll
-    for (int k = 0; k < V; ++k) g[k] = 0.f;
-    if (s < len) {
-      for (int j = 0; j < K; ++j) {
+    for (int k = 0; k < V; ++k) bias[k] = a.bias ? a.bias[c + k] : 0.f;
+  }
+  const bool linear = KIND == CLAMP && a.act.lo != a.act.lo;
+  const long jobs = on ? (long)a.B * runs : 0;
+  for (long job = (long)blockIdx.y * JY + ty; job < jobs; job += (long)gridDim.y * JY) {
+    const int b = (int)(job / runs), s0 = (int)(job % runs) * run, s1 = min(s0 + run, a.T);
+    const int len = seq_len(a, b);
+    const Line<const T> x = line(a, (const T*)a.x, a.ldx, b, c, len);
+    const Line<const T> dy = line(a, (const T*)a.dy, a.ldy, b, c, len);
+    const Line<T> dx = line(a, (T*)a.dx, (long)a.D, b, c, len);
+    Raw<T, V> win[KP - 1 + U];
+    float ew[KP][V];  // e at p - KP + 1 .. p
+#pragma unroll
+    for (int j = 0; j < KP - 1; ++j) input<T, V>(a, x, b, c, s0 - KP + 1 + j, len, win[j]);
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) ew[j][k] = 0.f;
+    const int end = s1 + K - 1;
+    for (int p0 = s0; p0 < end; p0 += U) {
+      Raw<T, V> g[U];
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        const int p = p0 + r;
+        if (p < end) input<T, V>(a, x, b, c, p, len, win[KP - 1 + r]);
+        if (p < end && p < len) g[r].load(dy.base + p * dy.step);
+        else g[r].zero();
+      }
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        const int p = p0 + r;
+        if (p >= end) break;
         float e[V];
-        pre_grad<T, V, KIND>(a, b, c, s + K - 1 - j, len, bias, e);
 #pragma unroll
-        for (int k = 0; k < V; ++k) g[k] = fmaf(a.w[(long)j * a.D + c + k], e[k], g[k]);
-      }
-      if (a.dxT && s >= len - (K - 1)) {
-        float v[V];
-        load_vec<T, V>((const T*)a.dxT + ((long)(s - len + K - 1) * a.B + b) * a.D + c, v);
+        for (int k = 0; k < V; ++k) e[k] = bias[k];
+        if (!linear)
 #pragma unroll
-        for (int k = 0; k < V; ++k) g[k] += v[k];
+          for (int j = 0; j < KP; ++j)
+            if (EXACT || j >= skip)
+#pragma unroll
+              for (int k = 0; k < V; ++k) e[k] = fmaf(w[j][k], win[r + j][k], e[k]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) e[k] = p < len ? g[r][k] * act_grad<KIND>(e[k], a.act) : 0.f;
+#pragma unroll
+        for (int j = 0; j < KP - 1; ++j)
+#pragma unroll
+          for (int k = 0; k < V; ++k) ew[j][k] = ew[j + 1][k];
+#pragma unroll
+        for (int k = 0; k < V; ++k) ew[KP - 1][k] = e[k];
+        if (p < s1 && p < len) {
+#pragma unroll
+          for (int j = 0; j < KP; ++j)
+            if (EXACT || j >= skip)
+#pragma unroll
+              for (int k = 0; k < V; ++k) dw[j][k] = fmaf(e[k], win[r + j][k], dw[j][k]);
+#pragma unroll
+          for (int k = 0; k < V; ++k) db[k] += e[k];
+        }
+        const int s = p - K + 1;
+        if (s >= s1 || (s < s0 && !(s0 == 0 && a.dx0))) continue;
+        float o[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] = 0.f;
+#pragma unroll
+        for (int j = 0; j < KP; ++j)  // tap j with e_{p - j}
+          if (EXACT || j < K)
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+              o[k] = fmaf(EXACT ? w[j][k] : wl[EXACT ? 0 : j][k], ew[KP - 1 - j][k], o[k]);
+        if (a.dxT && s < len && s >= len - (K - 1)) {
+          Raw<T, V> v;
+          v.load((const T*)a.dxT + ((long)(s - len + K - 1) * a.B + b) * a.D + c);
+#pragma unroll
+          for (int k = 0; k < V; ++k) o[k] += v[k];
+        }
+        T* at = s < 0 ? (T*)a.dx0 + ((long)(s + K - 1) * a.B + b) * a.D + c
+              : s < len ? dx.base + s * dx.step
+                        : (T*)a.dx + ((long)s * a.B + b) * a.D + c;
+        store_vec<T, V>(at, o);
       }
+#pragma unroll
+      for (int j = 0; j < KP - 1; ++j) win[j] = win[U + j];
     }
-    if (state) store_vec<T, V>((T*)a.dx0 + ((long)(s + K - 1) * a.B + b) * a.D + c, g);
-    else store_vec<T, V>((T*)a.dx + row_of(a, b, s, len) * a.D + c, g);
+  }
+  // the slab [K + 1][D] of this workgroup row
+#pragma unroll
+  for (int j = 0; j <= KP; ++j) {
+    if (j < KP && !EXACT && j < skip) continue;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < V; ++k) red[ty][cl * V + k] = j < KP ? dw[j < KP ? j : 0][k] : db[k];
+    __syncthreads();
+    for (int i = threadIdx.x; i < CX * V; i += 256) {
+      const int ch = blockIdx.x * CX * V + i;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < JY; ++r) sum += red[r][i];
+      if (ch < a.D) a.part[((long)blockIdx.y * (K + 1) + (j < KP ? j - skip : K)) * a.D + ch] = sum;
+    }
   }
 }
 
-// dw[k] = sum e_s x_{s - K + 1 + k}, dbias = sum e_s: a slab of jobs
-// (sequence, run) per workgroup row, no atomics.
-template <typename T, int V, int KIND>
-__global__ void __launch_bounds__(256) wgrad_k(Args a, int runs, int slabs) {
-  const int cv = a.D / V;
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i >= cv) return;
-  const int c = i * V, K = a.K;
-  float bias[V], acc[KMAX + 1][V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) bias[k] = a.bias ? a.bias[c + k] : 0.f;
-#pragma unroll
-  for (int j = 0; j <= KMAX; ++j)
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[j][k] = 0.f;
-  for (long job = blockIdx.y; job < (long)a.B * runs; job += slabs) {
-    const int b = (int)(job % a.B), s0 = (int)(job / a.B) * RUN, len = seq_len(a, b);
-    for (int s = s0; s < min(s0 + RUN, len); ++s) {
-      float e[V];
-      pre_grad<T, V, KIND>(a, b, c, s, len, bias, e);
-#pragma unroll
-      for (int k = 0; k < V; ++k) acc[KMAX][k] += e[k];
-#pragma unroll
-      for (int j = 0; j < KMAX; ++j) {
-        if (j >= K) break;
-        float v[V];
-        input<T, V>(a, b, c, s - K + 1 + j, len, v);
-#pragma unroll
-        for (int k = 0; k < V; ++k) acc[j][k] = fmaf(e[k], v[k], acc[j][k]);
-      }
-    }
-  }
-  float* out = a.part + (long)blockIdx.y * (K + 1) * a.D + c;
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-#pragma unroll
-    for (int j = 0; j < KMAX; ++j)
-      if (j < K) out[(long)j * a.D + k] = acc[j][k];
-    out[(long)K * a.D + k] = acc[KMAX][k];
-  }
-}
-
+// dw [K][D], dbias [D]: the sum over the slabs, 32 columns x 8 rows a workgroup
 __global__ void __launch_bounds__(256)
 param_grad_k(const float* __restrict__ p, int S, int K, int D, float* dw, float* db, int acc_w,
              int acc_b) {
+  __shared__ float red[8][33];
   const long total = (long)(K + 1) * D;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  float s = 0.f;
-  for (int k = 0; k < S; ++k) s += p[k * total + i];
+  const int cl = threadIdx.x % 32, r0 = threadIdx.x / 32;
+  const long i = (long)blockIdx.x * 32 + cl;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (i < total)
+    for (int r = r0; r < S; r += 32)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (r + 8 * k < S) s[k] += p[(long)(r + 8 * k) * total + i];
+  red[r0][cl] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (r0 || i >= total) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sum += red[r][cl];
   const bool isw = i < (long)K * D;
   float* out = isw ? dw : db;
   if (!out) return;
   out += isw ? i : i - (long)K * D;
-  *out = (isw ? acc_w : acc_b) ? *out + s : s;
+  *out = (isw ? acc_w : acc_b) ? *out + sum : sum;
 }
 
 // One token: y from the state and x, the state [K-1][B][D] moved on by one.
@@ -231,21 +308,44 @@ inline bool bad(const Args& a) {
   return a.T <= 0 || a.B <= 0 || a.D <= 0 || a.K < 1 || a.K > KMAX;
 }
 
-inline int slabs(long jobs) { return (int)(jobs < 256 ? jobs : 256); }
+// Positions of a thread's run: long runs read few rows twice, short ones fill the
+// card (2048 waves).
+inline int run_of(long T, long lanes) {
+  int run = 64;
+  while (run > 8 && lanes * ceil_div(T, run) < 2048 * 64) run /= 2;
+  return run;
+}
+
+constexpr int BV = 4, BCX = 32;  // backward: channels of a vector, vectors of a workgroup row
+
+inline int bwd_slabs(int T, int B, int D, int run) {
+  const long rows = ceil_div((long)B * ceil_div(T, run), 256 / BCX);
+  const long most = ceil_div(2048, ceil_div(D, BCX * BV));
+  return (int)(rows < most ? rows : most);
+}
 
 }  // namespace cconv
 }  // namespace kfb
 
 using namespace kfb;
 
-#define KFB_CCONV_VEC(T, vec, V, ...)                                     \
-  if (vec) { constexpr int V = 16 / sizeof(T); __VA_ARGS__; }              \
+#define KFB_CCONV_VEC(vec, WIDE, V, ...)         \
+  if (vec) { constexpr int V = WIDE; __VA_ARGS__; } \
   else { constexpr int V = 1; __VA_ARGS__; }
+
+// filter lengths: 2, 3 and 4 with everything unrolled, the others inside 8
+#define KFB_CCONV_TAPS(K, KP, EXACT, ...)                                  \
+  switch (K) {                                                             \
+    case 2: { constexpr int KP = 2; constexpr bool EXACT = true; __VA_ARGS__; break; } \
+    case 3: { constexpr int KP = 3; constexpr bool EXACT = true; __VA_ARGS__; break; } \
+    case 4: { constexpr int KP = 4; constexpr bool EXACT = true; __VA_ARGS__; break; } \
+    default: { constexpr int KP = 8; constexpr bool EXACT = false; __VA_ARGS__; break; } \
+  }
 
 KFB_API int kfb_cconv_max_taps() { return cconv::KMAX; }
 
 KFB_API long kfb_cconv_bwd_ws(int T, int B, int D, int K) {
-  return (long)cconv::slabs((long)B * ceil_div(T, cconv::RUN)) * (K + 1) * D;
+  return (long)cconv::bwd_slabs(T, B, D, cconv::run_of(T, (long)ceil_div(D, cconv::BV) * B)) * (K + 1) * D;
 }
 
 KFB_API hipError_t kfb_cconv_fwd(int dtype, int vec, const void* x, long ldx, const void* x0,
@@ -255,12 +355,17 @@ KFB_API hipError_t kfb_cconv_fwd(int dtype, int vec, const void* x, long ldx, co
   cconv::Args a{};
   a.x = x; a.ldx = ldx; a.x0 = x0; a.w = w; a.bias = bias; a.len = len; a.y = y; a.xT = xT;
   a.T = T; a.B = B; a.D = D; a.K = K; a.act = act_of(act); a.reverse = reverse;
-  const int runs = ceil_div(T, cconv::RUN);
-  if (cconv::bad(a) || runs > 65534) return hipErrorInvalidValue;
+  if (cconv::bad(a)) return hipErrorInvalidValue;
   KFB_DISPATCH_DTYPE(dtype, E, KFB_DISPATCH_ACT(a.act.kind, KIND, {
-    KFB_CCONV_VEC(E, vec, V, {
-      hipLaunchKernelGGL((cconv::fwd_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256), runs + (xT && K > 1 ? 1 : 0)),
-                         dim3(256), 0, stream, a, runs);
+    KFB_CCONV_VEC(vec, 16 / sizeof(E), V, {
+      const long lanes = (long)D / V * B;
+      const int run = cconv::run_of(T, lanes), runs = ceil_div(T, run);
+      if (runs > 65534 || lanes > (1l << 31)) return hipErrorInvalidValue;
+      KFB_CCONV_TAPS(K, KP, EXACT, {
+        hipLaunchKernelGGL((cconv::fwd_k<E, V, KIND, KP, EXACT>),
+                           dim3(ceil_div(lanes, 256), runs + (xT && K > 1 ? 1 : 0)), dim3(256), 0,
+                           stream, a, run, runs);
+      });
     });
   }));
   return hipGetLastError();
@@ -275,18 +380,19 @@ KFB_API hipError_t kfb_cconv_bwd(int dtype, int vec, const void* dy, long ldy, c
   a.dy = dy; a.ldy = ldy; a.x = x; a.ldx = ldx; a.x0 = x0; a.w = w; a.bias = bias; a.len = len;
   a.dxT = dxT; a.dx = dx; a.dx0 = dx0; a.part = ws;
   a.T = T; a.B = B; a.D = D; a.K = K; a.act = act_of(act); a.reverse = reverse;
-  const int runs = ceil_div(T, cconv::RUN);
-  if (cconv::bad(a) || runs > 65534 || !ws) return hipErrorInvalidValue;
-  const int S = cconv::slabs((long)B * runs);
+  if (cconv::bad(a) || !ws) return hipErrorInvalidValue;
+  const int run = cconv::run_of(T, (long)ceil_div(D, cconv::BV) * B), runs = ceil_div(T, run);
+  const int S = cconv::bwd_slabs(T, B, D, run);
   KFB_DISPATCH_DTYPE(dtype, E, KFB_DISPATCH_ACT(a.act.kind, KIND, {
-    KFB_CCONV_VEC(E, vec, V, {
-      hipLaunchKernelGGL((cconv::dgrad_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256), runs + (dx0 && K > 1 ? 1 : 0)),
-                         dim3(256), 0, stream, a, runs);
-      hipLaunchKernelGGL((cconv::wgrad_k<E, V, KIND>), dim3(ceil_div(D / V, 256), S), dim3(256), 0, stream,
-                         a, runs, S);
+    KFB_CCONV_VEC(vec, cconv::BV, V, {
+      // the same slabs for any vector width
+      KFB_CCONV_TAPS(K, KP, EXACT, {
+        hipLaunchKernelGGL((cconv::bwd_k<E, V, KIND, KP, EXACT, cconv::BCX>),
+                           dim3(ceil_div(D, cconv::BCX * V), S), dim3(256), 0, stream, a, run, runs);
+      });
     });
   }));
-  hipLaunchKernelGGL(cconv::param_grad_k, dim3(ceil_div((long)(K + 1) * D, 256)), dim3(256), 0,
+  hipLaunchKernelGGL(cconv::param_grad_k, dim3(ceil_div((long)(K + 1) * D, 32)), dim3(256), 0,
                      stream, ws, S, K, D, dw, db, acc_w, acc_b);
   return hipGetLastError();
 }
@@ -299,9 +405,9 @@ KFB_API hipError_t kfb_cconv_step(int dtype, int vec, const void* x, long ldx, v
   a.T = 1; a.B = B; a.D = D; a.K = K; a.act = act_of(act);
   if (cconv::bad(a)) return hipErrorInvalidValue;
   KFB_DISPATCH_DTYPE(dtype, E, KFB_DISPATCH_ACT(a.act.kind, KIND, {
-    KFB_CCONV_VEC(E, vec, V, {
-      hipLaunchKernelGGL((cconv::step_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256)), dim3(256), 0,
-                         stream, a, (E*)state);
+    KFB_CCONV_VEC(vec, 16 / sizeof(E), V, {
+      hipLaunchKernelGGL((cconv::step_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256)), dim3(256),
+                         0, stream, a, (E*)state);
     });
   }));
   return hipGetLastError();

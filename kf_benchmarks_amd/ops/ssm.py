@@ -177,9 +177,8 @@ class _CausalConv(torch.autograd.Function):
         dinit = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[3] else None
         grads, acc = _grad_buffers(ctx.params)
         ws = torch.empty((N.query("kfb_cconv_bwd_ws", T, B, D, K),), dtype=torch.float32, device=dev)
-        ve = 16 // x.element_size()
         N.call("kfb_cconv_bwd", N.dt(x),
-               int(_vec(D, ve, (x, ldx), (dy, ldy), (initial, D), (dlast, D))), dy.data_ptr(), ldy,
+               int(_vec(D, 4, (x, ldx), (dy, ldy), (initial, D), (dlast, D))), dy.data_ptr(), ldy,
                x.data_ptr(), ldx, N.ptr(initial), w.data_ptr(), N.ptr(b), N.ptr(lengths),
                N.ptr(dlast), dx.data_ptr(), N.ptr(dinit), N.ptr(grads[0]), N.ptr(grads[1]), acc[0],
                acc[1], ws.data_ptr(), T, B, D, K, act, int(reverse), N.stream(dev))
