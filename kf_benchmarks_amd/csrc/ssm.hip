@@ -12,8 +12,17 @@
 // scalar loads, from a copy in fp32 that is laid out per wave (prep_k).  A tile
 // of TQ steps is staged in LDS as (dt, dt x), the waves walk it with their
 // states in registers and leave their part of sum_n C h in LDS, and the tile's
-// elementwise end is again one pass over (step, channel).
+// elementwise end is again one pass over (step, channel).  The next tile's rows are
+// loaded while a tile is walked.
+//
+// Bound by the vector units: an exponential (8 cycles a wave) and four fused
+// operations (4 cycles each) per state, 24 cycles; the bytes take a quarter to
+// a half of that.  Where B D / 64 workgroups do not fill the card, a sequence is
+// cut into chunks: ends_k walks every chunk but the last from a zero state, and
+// because the decays of a chunk multiply to exp(A sum dt), the state before a
+// chunk follows from the earlier chunks' (end, sum dt) alone.
 #include "act.h"
+#include "raw.h"
 
 namespace kfb {
 namespace ssm {
@@ -33,11 +42,25 @@ struct Args {
   const float* dhT;  // [B][N][D] or null
   float* dh0;        // [B][N][D] or null
   float* pbc;        // [D / 64][T * B][2 N]
-  float* pch;        // [B][N + 2][D], dA | dskip | dbias of a sequence
+  float* pch;        // [B * nchunk][N + 2][D], dA | dskip | dbias of a chunk
+  // chunks of tpc tiles: end state (backward: gradient before the chunk) from
+  // zero [nchunk][B][N][D], sum of dt [nchunk][B][D]
+  float *ends, *sums;
+  int nchunk, tpc;
   int T, B, D, N, W, Tp, softplus, reverse;
 };
 
-template <int V> struct Pack { float v[V]; };
+// B and C as constant memory: uniform addresses become scalar loads
+typedef const __attribute__((address_space(4))) float cfloat;
+
+// The same address as a value the compiler does not know: loads through it are
+// neither merged with earlier ones nor moved up, which would keep more values
+// of B and C alive than there are scalar registers.
+__device__ __forceinline__ cfloat* fresh(const float* p) {
+  uintptr_t q = (uintptr_t)p;
+  asm volatile("" : "+s"(q));
+  return (cfloat*)q;
+}
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.T) : a.T;
@@ -70,277 +93,463 @@ __global__ void __launch_bounds__(256) prep_k(Args a) {
   }
 }
 
-template <typename T, int V, int NS, int TQ>
+// A thread's part of the elementwise passes over a tile: IT vectors of V channels,
+// the same channels in each (the thread count is a multiple of 64 / V).
+template <typename T, int V, int IT, int TQ> struct Part {
+  int r[IT];  // its steps of the tile (TQ: none)
+  int cl, c;  // its first channel: in the block, in the row
+  bool on;
+
+  __device__ __forceinline__ Part(const Args& a, int d0) {
+    cl = threadIdx.x % (64 / V) * V;
+    c = d0 + cl;
+    on = c < a.D;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int q = (threadIdx.x + i * a.W * 64) / (64 / V);
+      r[i] = q < TQ ? q : TQ;
+    }
+  }
+  // rows s0 + r of p (step elements apart, from position 0), zero past ``n``
+  __device__ __forceinline__ void load(const T* p, long step, int s0, int n, Raw<T, V> (&v)[IT]) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      if (on && r[i] < TQ && s0 + r[i] < n) v[i].load(p + (s0 + r[i]) * step + cl);
+      else v[i].zero();
+    }
+  }
+};
+
+// Position 0 of sequence b in a [T][B] tensor and the elements to the next.
+template <typename T>
+__device__ __forceinline__ const T* line(const Args& a, const void* p, long ld, int b, int d0,
+                                         int len, long& step) {
+  step = (long)a.B * ld;
+  const T* q = (const T*)p + (long)b * ld + d0;
+  if (a.reverse && len > 0) {
+    q += (len - 1) * step;
+    step = -step;
+  }
+  return q;
+}
+
+template <int V>
+__device__ __forceinline__ void params(const float* p, int c, bool on, float (&v)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = on && p ? p[c + k] : 0.f;
+}
+
+__device__ __forceinline__ float step_size(float raw, bool softplus) {
+  return softplus ? softplusf(raw) : raw;
+}
+
+// ENDS: only the state after each chunk, from zero, and the chunk's sum of dt.
+template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   extern __shared__ float lds[];
+  constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;  // steps whose B and C are in scalar registers
   float2* du = (float2*)lds;           // [TQ][64]
   float* yp = lds + TQ * 64 * 2;       // [W][TQ][64]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane;
-  const int len = seq_len(a, b), nt = a.W * 64;
+  const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane, chunk = blockIdx.z;
+  const int len = seq_len(a, b);
+  const long bnd = ((long)b * a.N + w * NS) * a.D + d, bn = (long)a.B * a.N * a.D;
   float A2[NS], h[NS];
+  bool on[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    const int n = w * NS + i;
-    const bool on = n < a.N && d < a.D;
-    A2[i] = on ? a.A[(long)n * a.D + d] * LOG2E : 0.f;
-    h[i] = on && a.h0 ? a.h0[((long)b * a.N + n) * a.D + d] : 0.f;
+    on[i] = w * NS + i < a.N && d < a.D;
+    A2[i] = on[i] ? a.A[(long)(w * NS + i) * a.D + d] * LOG2E : 0.f;
+    h[i] = on[i] && a.h0 && !ENDS ? a.h0[bnd + (long)i * a.D] : 0.f;
   }
-  const float* __restrict__ bcw = a.bc + ((long)b * a.W + w) * a.Tp * 2 * NS;
-  for (int s0 = 0; s0 < a.T; s0 += TQ) {
-    for (int i = threadIdx.x; i < TQ * 64 / V; i += nt) {
-      const int r = i / (64 / V), cl = i % (64 / V) * V, c = d0 + cl, s = s0 + r;
-      float xv[V], dv[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) xv[k] = dv[k] = 0.f;
-      if (s < len && c < a.D) {
-        const long row = row_of(a, b, s, len);
-        load_vec<T, V>((const T*)a.x + row * a.ldx + c, xv);
-        load_vec<T, V>((const T*)a.delta + row * a.ldd + c, dv);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float raw = dv[k] + (a.bias ? a.bias[c + k] : 0.f);
-          dv[k] = a.softplus ? softplusf(raw) : raw;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) du[r * 64 + cl + k] = make_float2(dv[k], dv[k] * xv[k]);
-    }
-    if (a.hs && d < a.D) {
-      float* hs = a.hs + ((long)(s0 / TQ) * a.B + b) * a.N * a.D + d;
+  if constexpr (!ENDS)
+    for (int j = 0; j < chunk; ++j) {
+      const float sum = d < a.D ? a.sums[((long)j * a.B + b) * a.D + d] : 0.f;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
-        if (w * NS + i < a.N) hs[(long)(w * NS + i) * a.D] = h[i];
+        if (on[i])
+          h[i] = fmaf(__builtin_amdgcn_exp2f(sum * A2[i]), h[i], a.ends[j * bn + bnd + (long)i * a.D]);
     }
-    __syncthreads();
-    const float* __restrict__ bct = bcw + (long)s0 * 2 * NS;
-#pragma unroll 4
-    for (int r = 0; r < TQ; ++r) {
-      const float2 u = du[r * 64 + lane];
-      float v = 0.f;
+  const float* bcw = a.bc + ((long)b * a.W + w) * a.Tp * 2 * NS;
+  const Part<T, V, IT, TQ> me(a, d0);
+  long stx, std, stz = 0;
+  const T* px = line<T>(a, a.x, a.ldx, b, d0, len, stx);
+  const T* pd = line<T>(a, a.delta, a.ldd, b, d0, len, std);
+  const T* pz = a.z ? line<T>(a, a.z, a.ldz, b, d0, len, stz) : px;
+  float bias[V], skip[V];
+  params<V>(a.bias, me.c, me.on, bias);
+  params<V>(a.skip, me.c, me.on, skip);
+  Raw<T, V> nx[IT], nd[IT], nz[IT], cx[IT], cz[IT];
+  const int s_end = min((chunk + 1) * a.tpc * TQ, a.Tp);
+  auto fetch = [&](int s0) {
+    me.load(px, stx, s0, len, nx);
+    me.load(pd, std, s0, len, nd);
+    if (!ENDS && a.z) me.load(pz, stz, s0, len, nz);
+  };
+  auto stage = [&](int s0) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        h[i] = fmaf(__builtin_amdgcn_exp2f(u.x * A2[i]), h[i], u.y * bct[r * 2 * NS + i]);
-        v = fmaf(bct[r * 2 * NS + NS + i], h[i], v);
-      }
-      yp[(w * TQ + r) * 64 + lane] = v;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < TQ * 64 / V; i += nt) {
-      const int r = i / (64 / V), cl = i % (64 / V) * V, c = d0 + cl, s = s0 + r;
-      if (s >= a.T || c >= a.D) continue;
-      const long row = row_of(a, b, s, len);
-      float v[V], xv[V], zv[V];
+    for (int i = 0; i < IT; ++i) {
+      if (me.r[i] < TQ) {
+        const bool in = me.on && s0 + me.r[i] < len;
 #pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = 0.f;
-      if (s < len) {
-        for (int q = 0; q < a.W; ++q) {
-          const Pack<V> p = *(const Pack<V>*)(yp + (q * TQ + r) * 64 + cl);
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] += p.v[k];
-        }
-        if (a.skip) {
-          load_vec<T, V>((const T*)a.x + row * a.ldx + c, xv);
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = fmaf(a.skip[c + k], xv[k], v[k]);
-        }
-        if (a.z) {
-          load_vec<T, V>((const T*)a.z + row * a.ldz + c, zv);
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] *= siluf(zv[k]);
+        for (int k = 0; k < V; ++k) {
+          const float dt = in ? step_size(nd[i][k] + bias[k], a.softplus) : 0.f;
+          du[me.r[i] * 64 + me.cl + k] = make_float2(dt, dt * nx[i][k]);
         }
       }
-      store_vec<T, V>((T*)a.y + row * a.D + c, v);
+      cx[i] = nx[i];
+      cz[i] = nz[i];
     }
+  };
+  float sum_dt = 0.f;
+  int s0 = chunk * a.tpc * TQ;
+  fetch(s0);
+  stage(s0);
+  __syncthreads();
+  for (; s0 < s_end; s0 += TQ) {
+    const bool more = s0 + TQ < s_end;
+    if (more) fetch(s0 + TQ);
+    if (!ENDS && a.hs) {
+      float* hs = a.hs + (long)(s0 / TQ) * bn + bnd;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (on[i]) hs[(long)i * a.D] = h[i];
+    }
+#pragma unroll
+    for (int r0 = 0; r0 < TQ; r0 += UR) {
+      cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+#pragma unroll
+      for (int k = 0; k < UR; ++k) {
+        const float2 u = du[(r0 + k) * 64 + lane];
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          h[i] = fmaf(__builtin_amdgcn_exp2f(u.x * A2[i]), h[i], u.y * bct[k * 2 * NS + i]);
+          if (!ENDS) v = fmaf(bct[k * 2 * NS + NS + i], h[i], v);
+        }
+        if constexpr (ENDS) sum_dt += u.x;
+        else yp[(w * TQ + r0 + k) * 64 + lane] = v;
+      }
+    }
+    __syncthreads();
+    if constexpr (!ENDS) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int r = me.r[i], s = s0 + r;
+        if (r >= TQ || s >= a.T || !me.on) continue;
+        float v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = skip[k] * cx[i][k];
+        for (int q = 0; q < a.W; ++q)
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] += yp[(q * TQ + r) * 64 + me.cl + k];
+        if (a.z)
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] *= siluf(cz[i][k]);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = s < len ? v[k] : 0.f;
+        store_vec<T, V>((T*)a.y + row_of(a, b, s, len) * a.D + me.c, v);
+      }
+    }
+    if (more) stage(s0 + TQ);
+    __syncthreads();
   }
-  if (a.hT && d < a.D)
+  if constexpr (ENDS) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      if (w * NS + i < a.N) a.hT[((long)b * a.N + w * NS + i) * a.D + d] = h[i];
+      if (on[i]) a.ends[chunk * bn + bnd + (long)i * a.D] = h[i];
+    if (w == 0 && d < a.D) a.sums[((long)chunk * a.B + b) * a.D + d] = sum_dt;
+  } else if (a.hT && chunk == a.nchunk - 1) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+      if (on[i]) a.hT[bnd + (long)i * a.D] = h[i];
+  }
 }
 
-// Backward: the tiles from the last to the first, each one first forward again
-// from its saved state (the TQ states and decays stay in registers), then back:
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL,
+                                                               0xf, 0xf, true));
+}
+
+// Sums over the wave's lanes of M = 2, 4, 8 or 16 values at once, halving the
+// number of registers where it halves the lanes: 18 instructions for 8 values
+// instead of 48.  Lane l ends up with the sum of value lane_value<M>(l).
+template <int M> __device__ __forceinline__ float lanes_sum(float (&v)[M], int lane) {
+  static_assert(M == 2 || M == 4 || M == 8 || M == 16, "2, 4, 8 or 16 values");
+#pragma unroll
+  for (int i = 0; i < M / 2; ++i) {  // lanes 0-31 | 32-63
+    const auto q = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v[i]),
+                                                    __builtin_bit_cast(unsigned, v[i + M / 2]), false, false);
+    const unsigned lo = q[0], hi = q[1];  // (a bit_cast of q[1] itself takes element 0)
+    v[i] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+  }
+  constexpr int R = M / 4 > 0 ? M / 4 : 1;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {  // even | odd rows of 16 (M = 2: the sum is left in the even ones)
+    const auto q = __builtin_amdgcn_permlane16_swap(
+        __builtin_bit_cast(unsigned, v[i]), M == 2 ? 0u : __builtin_bit_cast(unsigned, v[i + R < M ? i + R : 0]),
+        false, false);
+    const unsigned lo = q[0], hi = q[1];  // (a bit_cast of q[1] itself takes element 0)
+    v[i] = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+  }
+  const bool b3 = lane & 8, b2 = lane & 4;
+  if constexpr (M >= 8) {
+#pragma unroll
+    for (int i = 0; i < M / 8; ++i)  // lane ^ 8: row_ror:8
+      v[i] = (b3 ? v[2 * i + 1] : v[2 * i]) + dpp<0x128>(b3 ? v[2 * i] : v[2 * i + 1]);
+  } else {
+    v[0] += dpp<0x128>(v[0]);
+  }
+  float s;
+  if constexpr (M == 16) s = (b2 ? v[1] : v[0]) + dpp<0x141>(b2 ? v[0] : v[1]);  // lane ^ 7: row_half_mirror
+  else s = v[0] + dpp<0x141>(v[0]);
+  s += dpp<0xB1>(s);  // lane ^ 1
+  s += dpp<0x4E>(s);  // lane ^ 2
+  return s;
+}
+
+template <int M> __device__ __forceinline__ int lane_value(int l) {
+  const int b2 = l >> 2 & 1, b3 = l >> 3 & 1, row = l >> 4;
+  switch (M) {
+    case 2: return row >> 1;
+    case 4: return (row & 1) + 2 * (row >> 1);
+    case 8: return b3 + 2 * (row & 1) + 4 * (row >> 1);
+    default: return b3 + 2 * b2 + 4 * (row & 1) + 8 * (row >> 1);
+  }
+}
+
+// Backward.  The tiles of a chunk from the last to the first, each one first
+// forward again from its saved state (the TQ states and decays stay in registers),
+// then back:
 //   g = C e + a_{t+1} g_{t+1},  e = dy silu(z)
 //   p = sum_n g B, q = sum_n g A a h_{t-1}:  dx = dt p + skip e, ddt = q + x p
 //   dA = sum_t g dt a h_{t-1};  dB = sum_d g dt x;  dC = sum_d e h.
 // dB and dC are summed over the wave's 64 channels here and over the channel
-// blocks by bc_grad_k, dA, dskip and dbias over the sequences by
-// param_grad_k: no atomics, the same sums on every run.
-template <typename T, int V, int NS, int TQ>
+// blocks by bc_grad_k, dA, dskip and dbias over the chunks by param_grad_k: no
+// atomics, the same sums on every run.
+// ENDS: only the gradient before each chunk, from zero behind it, and sum dt.
+template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   extern __shared__ float lds[];
-  float* sd = lds;                         // [TQ][64] dt
-  float* sx = sd + TQ * 64;                // [TQ][64] dt x
-  float* se = sx + TQ * 64;                // [TQ][64] e
-  float* yp = se + TQ * 64;                // [W][TQ][64]
-  float2* pq = (float2*)(yp + a.W * TQ * 64);  // [W][TQ][64]
+  const int WN = a.W * NS;
+  constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;
+  float2* du = (float2*)lds;                    // [TQ][64] dt, dt x
+  float* se = lds + TQ * 64 * 2;                // [TQ][64] e
+  float* sbc = se + TQ * 64;                    // [TQ][2 WN]
+  float* yp = sbc + TQ * 2 * WN;                // [W][TQ][64]
+  float2* pq = (float2*)(yp + a.W * TQ * 64);   // [W][TQ][64]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane;
+  const int chunk = ENDS ? blockIdx.z + 1 : blockIdx.z;
   const int len = seq_len(a, b), nt = a.W * 64;
+  const long bnd = ((long)b * a.N + w * NS) * a.D + d, bn = (long)a.B * a.N * a.D;
   float A1[NS], carry[NS], dA[NS];
-  constexpr int CH = V;  // channels of a thread in the elementwise passes
-  float gskip[CH], gbias[CH];
-#pragma unroll
-  for (int k = 0; k < CH; ++k) gskip[k] = gbias[k] = 0.f;
+  bool on[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    const int n = w * NS + i;
-    const bool on = n < a.N && d < a.D;
-    A1[i] = on ? a.A[(long)n * a.D + d] : 0.f;
-    carry[i] = on && a.dhT ? a.dhT[((long)b * a.N + n) * a.D + d] : 0.f;
+    on[i] = w * NS + i < a.N && d < a.D;
+    A1[i] = on[i] ? a.A[(long)(w * NS + i) * a.D + d] : 0.f;
+    carry[i] = on[i] && a.dhT && !ENDS ? a.dhT[bnd + (long)i * a.D] : 0.f;
     dA[i] = 0.f;
   }
-  const float* __restrict__ bcw = a.bc + ((long)b * a.W + w) * a.Tp * 2 * NS;
-  const int ntile = a.Tp / TQ;
-  for (int tile = ntile - 1; tile >= 0; --tile) {
-    const int s0 = tile * TQ;
-    for (int i = threadIdx.x; i < TQ * 64 / V; i += nt) {
-      const int r = i / (64 / V), cl = i % (64 / V) * V, c = d0 + cl, s = s0 + r;
-      float xv[V], dv[V], ev[V], zv[V];
+  if constexpr (!ENDS)
+    for (int j = a.nchunk - 1; j > chunk; --j) {
+      const float sum = d < a.D ? a.sums[((long)j * a.B + b) * a.D + d] : 0.f;
 #pragma unroll
-      for (int k = 0; k < V; ++k) xv[k] = dv[k] = ev[k] = 0.f;
-      if (s < len && c < a.D) {
-        const long row = row_of(a, b, s, len);
-        load_vec<T, V>((const T*)a.x + row * a.ldx + c, xv);
-        load_vec<T, V>((const T*)a.delta + row * a.ldd + c, dv);
-        load_vec<T, V>((const T*)a.dy + row * a.ldy + c, ev);
+      for (int i = 0; i < NS; ++i)
+        if (on[i])
+          carry[i] = fmaf(__builtin_amdgcn_exp2f(sum * (A1[i] * LOG2E)), carry[i],
+                          a.ends[j * bn + bnd + (long)i * a.D]);
+    }
+  const float* bcw = a.bc + ((long)b * a.W + w) * a.Tp * 2 * NS;
+  const Part<T, V, IT, TQ> me(a, d0);
+  long stx, std, sty, stz = 0;
+  const T* px = line<T>(a, a.x, a.ldx, b, d0, len, stx);
+  const T* pd = line<T>(a, a.delta, a.ldd, b, d0, len, std);
+  const T* py = line<T>(a, a.dy, a.ldy, b, d0, len, sty);
+  const T* pz = a.z ? line<T>(a, a.z, a.ldz, b, d0, len, stz) : px;
+  float bias[V], skip[V], gskip[V], gbias[V];
+  params<V>(a.bias, me.c, me.on, bias);
+  params<V>(a.skip, me.c, me.on, skip);
+#pragma unroll
+  for (int k = 0; k < V; ++k) gskip[k] = gbias[k] = 0.f;
+  Raw<T, V> nx[IT], nd[IT], ny[IT], nz[IT], cx[IT], cd[IT], cy[IT], cz[IT];
+  auto fetch = [&](int s0) {
+    if (!ENDS) me.load(px, stx, s0, len, nx);
+    me.load(pd, std, s0, len, nd);
+    me.load(py, sty, s0, len, ny);
+    if (a.z) me.load(pz, stz, s0, len, nz);
+  };
+  auto stage = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      if (me.r[i] < TQ) {
+        const bool in = me.on && s0 + me.r[i] < len;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float raw = dv[k] + (a.bias ? a.bias[c + k] : 0.f);
-          dv[k] = a.softplus ? softplusf(raw) : raw;
-        }
-        if (a.z) {
-          load_vec<T, V>((const T*)a.z + row * a.ldz + c, zv);
-#pragma unroll
-          for (int k = 0; k < V; ++k) ev[k] *= siluf(zv[k]);
+          const float dt = in ? step_size(nd[i][k] + bias[k], a.softplus) : 0.f;
+          du[me.r[i] * 64 + me.cl + k] = make_float2(dt, ENDS ? 0.f : dt * nx[i][k]);
+          se[me.r[i] * 64 + me.cl + k] = a.z ? ny[i][k] * siluf(nz[i][k]) : ny[i][k];
         }
       }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        sd[r * 64 + cl + k] = dv[k];
-        sx[r * 64 + cl + k] = dv[k] * xv[k];
-        se[r * 64 + cl + k] = ev[k];
-      }
+      cx[i] = nx[i];
+      cd[i] = nd[i];
+      cy[i] = ny[i];
+      cz[i] = nz[i];
     }
-    float hb[NS], H[TQ][NS], dec[TQ][NS];
-    const float* hs = a.hs + ((long)tile * a.B + b) * a.N * a.D + d;
+  };
+  // where a lane's sum of lanes_sum goes in a row of sbc
+  const int val = lane_value<2 * NS>(lane);
+  const int col = val < NS ? w * NS + val : WN + w * NS + val - NS;
+  const bool writer = (lane & (32 / NS - 1)) == 0;
+  const int t0 = chunk * a.tpc, t1 = min(t0 + a.tpc, a.Tp / TQ);
+  float sum_dt = 0.f;
+  fetch((t1 - 1) * TQ);
+  stage((t1 - 1) * TQ);
+  __syncthreads();
+  for (int tile = t1 - 1; tile >= t0; --tile) {
+    const int s0 = tile * TQ;
+    if (tile > t0) fetch(s0 - TQ);
+    if constexpr (ENDS) {
+#pragma unroll
+      for (int r0 = TQ - UR; r0 >= 0; r0 -= UR) {
+        cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+#pragma unroll
+        for (int k = UR - 1; k >= 0; --k) {
+          const float dt = du[(r0 + k) * 64 + lane].x, e = se[(r0 + k) * 64 + lane];
+          sum_dt += dt;
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+            carry[i] = fmaf(bct[k * 2 * NS + NS + i], e, carry[i]) *
+                       __builtin_amdgcn_exp2f(dt * (A1[i] * LOG2E));
+        }
+      }
+      __syncthreads();
+    } else {
+      float hb[NS], H[TQ][NS], dec[TQ][NS], dAt[NS];
+      const float* hs = a.hs + (long)tile * bn + bnd;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        hb[i] = on[i] ? hs[(long)i * a.D] : 0.f;
+        dAt[i] = 0.f;
+      }
+#pragma unroll
+      for (int r0 = 0; r0 < TQ; r0 += UR) {
+        cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+#pragma unroll
+        for (int k = 0; k < UR; ++k) {
+          const int r = r0 + k;
+          const float2 u = du[r * 64 + lane];
+          float v = 0.f;
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            dec[r][i] = __builtin_amdgcn_exp2f(u.x * (A1[i] * LOG2E));
+            H[r][i] = fmaf(dec[r][i], r ? H[r - 1][i] : hb[i], u.y * bct[k * 2 * NS + i]);
+            v = fmaf(bct[k * 2 * NS + NS + i], H[r][i], v);
+          }
+          if (a.z) yp[(w * TQ + r) * 64 + lane] = v;
+        }
+      }
+#pragma unroll
+      for (int r0 = TQ - UR; r0 >= 0; r0 -= UR) {
+        cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+#pragma unroll
+        for (int k = UR - 1; k >= 0; --k) {
+          const int r = r0 + k;
+          const float2 u = du[r * 64 + lane];
+          const float e = se[r * 64 + lane];
+          float p = 0.f, q = 0.f, red[2 * NS];
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            const float g = fmaf(bct[k * 2 * NS + NS + i], e, carry[i]);
+            p = fmaf(g, bct[k * 2 * NS + i], p);
+            red[i] = g * u.y;
+            red[NS + i] = e * H[r][i];
+            carry[i] = g * dec[r][i];
+            const float t = carry[i] * (r ? H[r - 1][i] : hb[i]);
+            q = fmaf(t, A1[i], q);
+            dAt[i] = fmaf(t, u.x, dAt[i]);
+          }
+          pq[(w * TQ + r) * 64 + lane] = make_float2(p, q);
+          const float s = lanes_sum<2 * NS>(red, lane);
+          if (writer) sbc[r * 2 * WN + col] = s;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i) dA[i] += dAt[i];
+      __syncthreads();
+      for (int i = threadIdx.x; i < TQ * 2 * a.N; i += nt) {
+        const int r = i / (2 * a.N), j = i - r * 2 * a.N, s = s0 + r;
+        if (s < a.T)
+          a.pbc[((long)blockIdx.x * a.T * a.B + row_of(a, b, s, len)) * 2 * a.N + j] =
+              sbc[r * 2 * WN + (j < a.N ? j : WN + j - a.N)];
+      }
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int r = me.r[i], s = s0 + r;
+        if (r >= TQ || s >= a.T || !me.on) continue;
+        float ox[V], od[V], oz[V];
+        const bool in = s < len;
+        float p[V], q[V], v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) p[k] = q[k] = v[k] = 0.f;
+        for (int u = 0; u < a.W; ++u)
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const float2 t = pq[(u * TQ + r) * 64 + me.cl + k];
+            p[k] += t.x;
+            q[k] += t.y;
+            if (a.z) v[k] += yp[(u * TQ + r) * 64 + me.cl + k];
+          }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float x = cx[i][k], e = se[r * 64 + me.cl + k], dt = du[r * 64 + me.cl + k].x;
+          float dd = fmaf(x, p[k], q[k]);
+          if (a.softplus) dd *= sigmoidf(cd[i][k] + bias[k]);
+          ox[k] = in ? fmaf(dt, p[k], skip[k] * e) : 0.f;
+          od[k] = in ? dd : 0.f;
+          oz[k] = in && a.z ? cy[i][k] * fmaf(skip[k], x, v[k]) * dsiluf(cz[i][k]) : 0.f;
+          gskip[k] = fmaf(e, x, gskip[k]);
+          gbias[k] += od[k];
+        }
+        const long at = row_of(a, b, s, len) * a.D + me.c;
+        store_vec<T, V>((T*)a.dx + at, ox);
+        store_vec<T, V>((T*)a.ddelta + at, od);
+        if (a.z) store_vec<T, V>((T*)a.dz + at, oz);
+      }
+      __syncthreads();
+    }
+    if (tile > t0) stage(s0 - TQ);
+    __syncthreads();
+  }
+  if constexpr (ENDS) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      hb[i] = w * NS + i < a.N && d < a.D ? hs[(long)(w * NS + i) * a.D] : 0.f;
-    __syncthreads();
-    const float* __restrict__ bct = bcw + (long)s0 * 2 * NS;
-#pragma unroll
-    for (int r = 0; r < TQ; ++r) {
-      const float dt = sd[r * 64 + lane], dtx = sx[r * 64 + lane];
-      float v = 0.f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        dec[r][i] = __builtin_amdgcn_exp2f(dt * (A1[i] * LOG2E));
-        H[r][i] = fmaf(dec[r][i], r ? H[r - 1][i] : hb[i], dtx * bct[r * 2 * NS + i]);
-        v = fmaf(bct[r * 2 * NS + NS + i], H[r][i], v);
-      }
-      if (a.z) yp[(w * TQ + r) * 64 + lane] = v;
-    }
-    float dAt[NS];
-#pragma unroll
-    for (int i = 0; i < NS; ++i) dAt[i] = 0.f;
-#pragma unroll
-    for (int r = TQ - 1; r >= 0; --r) {
-      const float dt = sd[r * 64 + lane], dtx = sx[r * 64 + lane], e = se[r * 64 + lane];
-      float p = 0.f, q = 0.f, red[2 * NS];
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const float g = fmaf(bct[r * 2 * NS + NS + i], e, carry[i]);
-        p = fmaf(g, bct[r * 2 * NS + i], p);
-        red[i] = g * dtx;
-        red[NS + i] = e * H[r][i];
-        carry[i] = g * dec[r][i];
-        const float k = carry[i] * (r ? H[r - 1][i] : hb[i]);
-        q = fmaf(k, A1[i], q);
-        dAt[i] = fmaf(k, dt, dAt[i]);
-      }
-      pq[(w * TQ + r) * 64 + lane] = make_float2(p, q);
-      const int s = s0 + r;
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) red[i] = wave_sum(red[i]);
-      if (s < a.T && lane == 0) {
-        float* out = a.pbc + ((long)blockIdx.x * a.T * a.B + row_of(a, b, s, len)) * 2 * a.N;
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-          if (w * NS + i < a.N) {
-            out[w * NS + i] = red[i];
-            out[a.N + w * NS + i] = red[NS + i];
-          }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < NS; ++i) dA[i] += dAt[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < TQ * 64 / V; i += nt) {
-      const int r = i / (64 / V), cl = i % (64 / V) * V, c = d0 + cl, s = s0 + r;
-      if (s >= a.T || c >= a.D) continue;
-      const long row = row_of(a, b, s, len);
-      float ox[V], od[V], oz[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) ox[k] = od[k] = oz[k] = 0.f;
-      if (s < len) {
-        float xv[V], dv[V], zv[V], gv[V];
-        load_vec<T, V>((const T*)a.x + row * a.ldx + c, xv);
-        load_vec<T, V>((const T*)a.delta + row * a.ldd + c, dv);
-        if (a.z) {
-          load_vec<T, V>((const T*)a.z + row * a.ldz + c, zv);
-          load_vec<T, V>((const T*)a.dy + row * a.ldy + c, gv);
-        }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          float p = 0.f, q = 0.f, v = 0.f;
-          for (int u = 0; u < a.W; ++u) {
-            const float2 t = pq[(u * TQ + r) * 64 + cl + k];
-            p += t.x;
-            q += t.y;
-            if (a.z) v += yp[(u * TQ + r) * 64 + cl + k];
-          }
-          const float sk = a.skip ? a.skip[c + k] : 0.f;
-          const float e = se[r * 64 + cl + k], dt = sd[r * 64 + cl + k];
-          ox[k] = fmaf(dt, p, sk * e);
-          float dd = fmaf(xv[k], p, q);
-          if (a.softplus) dd *= sigmoidf(dv[k] + (a.bias ? a.bias[c + k] : 0.f));
-          od[k] = dd;
-          if (a.z) oz[k] = gv[k] * fmaf(sk, xv[k], v) * dsiluf(zv[k]);
-          gskip[k] = fmaf(e, xv[k], gskip[k]);
-          gbias[k] += dd;
-        }
-      }
-      store_vec<T, V>((T*)a.dx + row * a.D + c, ox);
-      store_vec<T, V>((T*)a.ddelta + row * a.D + c, od);
-      if (a.z) store_vec<T, V>((T*)a.dz + row * a.D + c, oz);
-    }
-    __syncthreads();
+      if (on[i]) a.ends[chunk * bn + bnd + (long)i * a.D] = carry[i];
+    if (w == 0 && d < a.D) a.sums[((long)chunk * a.B + b) * a.D + d] = sum_dt;
+    return;
   }
-  float* pch = a.pch + (long)b * (a.N + 2) * a.D;
+  float* pch = a.pch + ((long)chunk * a.B + b) * (a.N + 2) * a.D;
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    const int n = w * NS + i;
-    if (n < a.N && d < a.D) {
-      pch[(long)n * a.D + d] = dA[i];
-      if (a.dh0) a.dh0[((long)b * a.N + n) * a.D + d] = carry[i];
+    if (on[i]) {
+      pch[(long)(w * NS + i) * a.D + d] = dA[i];
+      if (a.dh0 && chunk == 0) a.dh0[bnd + (long)i * a.D] = carry[i];
     }
   }
-  // dskip, dbias: thread i holds V channels (i % (64 / V)) of some rows
-  const int ncol = 64 / V, nrow = nt / ncol;
-  float* rs = lds;
+  // dskip, dbias: a thread holds V channels of some rows
+  const int nrow = nt / (64 / V), row = threadIdx.x / (64 / V);
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    rs[(threadIdx.x / ncol) * 64 + threadIdx.x % ncol * V + k] = gskip[k];
-    rs[(nrow + threadIdx.x / ncol) * 64 + threadIdx.x % ncol * V + k] = gbias[k];
+    lds[row * 64 + me.cl + k] = gskip[k];
+    lds[(nrow + row) * 64 + me.cl + k] = gbias[k];
   }
   __syncthreads();
   if (w == 0 && d < a.D) {
     float u = 0.f, v = 0.f;
     for (int r = 0; r < nrow; ++r) {
-      u += rs[r * 64 + lane];
-      v += rs[(nrow + r) * 64 + lane];
+      u += lds[r * 64 + lane];
+      v += lds[(nrow + r) * 64 + lane];
     }
     pch[(long)a.N * a.D + d] = u;
     pch[(long)(a.N + 1) * a.D + d] = v;
@@ -354,29 +563,44 @@ bc_grad_k(const float* __restrict__ p, int nblk, long rows, int N, T* __restrict
           T* __restrict__ dc) {
   const long total = rows * 2 * N;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    float s = 0.f;
-    for (int k = 0; k < nblk; ++k) s += p[k * total + i];
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < nblk; k += 4)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (k + u < nblk) s[u] += p[(k + u) * total + i];
     const long row = i / (2 * N);
     const int n = (int)(i % (2 * N));
-    (n < N ? db : dc)[row * N + (n < N ? n : n - N)] = from_f32<T>(s);
+    (n < N ? db : dc)[row * N + (n < N ? n : n - N)] = from_f32<T>((s[0] + s[1]) + (s[2] + s[3]));
   }
 }
 
-// dA [N][D], dskip, dbias [D]: the sum over the slabs of pch [S][N + 2][D]
+// dA [N][D], dskip, dbias [D]: the sum over the slabs of pch [S][N + 2][D], 32
+// columns x 8 rows a workgroup
 __global__ void __launch_bounds__(256)
 param_grad_k(const float* __restrict__ p, int S, int N, int D, float* dA, float* dskip,
              float* dbias, int acc_a, int acc_s, int acc_b) {
+  __shared__ float red[8][33];
   const long total = (long)(N + 2) * D;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  float s = 0.f;
-  for (int k = 0; k < S; ++k) s += p[k * total + i];
+  const int cl = threadIdx.x % 32, r0 = threadIdx.x / 32;
+  const long i = (long)blockIdx.x * 32 + cl;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (i < total)
+    for (int r = r0; r < S; r += 32)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (r + 8 * k < S) s[k] += p[(long)(r + 8 * k) * total + i];
+  red[r0][cl] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (r0 || i >= total) return;
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) sum += red[r][cl];
   const int n = (int)(i / D);
   float* out = n < N ? dA : n == N ? dskip : dbias;
   const int acc = n < N ? acc_a : n == N ? acc_s : acc_b;
   if (!out) return;
   out += n < N ? i : i % D;
-  *out = acc ? *out + s : s;
+  *out = acc ? *out + sum : sum;
 }
 
 // One token: state [B][N][D] in place.  64 channels x 4 waves, wave w the
@@ -415,20 +639,40 @@ __global__ void __launch_bounds__(256) step_k(Args a, float* __restrict__ state)
 
 struct Plan {
   int ns, tq, W, Tp, tiles;
+  int fc, bc;  // chunks of the forward and of the backward
 };
 
-inline Plan plan(int T, int N) {
+// A sequence is cut where its workgroups alone leave the card idle: up to
+// ``want`` workgroups, each at least 4 tiles long.
+inline int chunks_of(long wgs, int tiles, long want) {
+  long c = wgs >= want / 2 ? 1 : want / wgs;
+  if (c > tiles / 4) c = tiles / 4;
+  return (int)(c < 1 ? 1 : c > 65535 ? 65535 : c);
+}
+
+inline Plan plan(int T, int B, int D, int N) {
   Plan p;
-  p.ns = N <= 32 ? 4 : 8;
+  p.ns = N <= 4 ? 1 : N <= 8 ? 2 : N <= 32 ? 4 : 8;
   p.tq = N <= 32 ? 16 : 8;
   p.W = ceil_div(N, p.ns);
+  if (p.W < 4) p.W = 4;  // the elementwise passes want the threads
   p.tiles = ceil_div(T, p.tq);
   p.Tp = p.tiles * p.tq;
+  const long wgs = (long)ceil_div(D, 64) * B;
+  p.fc = chunks_of(wgs, p.tiles, 1024);
+  p.bc = chunks_of(wgs, p.tiles, 512);
   return p;
 }
 
+// tiles of a chunk; the count may come out smaller than asked for
+inline void cut(Args& a, const Plan& p, int chunks) {
+  a.tpc = ceil_div(p.tiles, chunks);
+  a.nchunk = ceil_div(p.tiles, a.tpc);
+}
+
 inline bool bad(const Args& a) {
-  return a.T <= 0 || a.B <= 0 || a.D <= 0 || a.N <= 0 || a.N > 64 || a.B > 65535;
+  return a.T <= 0 || a.B <= 0 || a.D <= 0 || a.N <= 0 || a.N > 64 || a.B > 65535 ||
+         a.T > INT32_MAX - 64;
 }
 
 }  // namespace ssm
@@ -436,56 +680,70 @@ inline bool bad(const Args& a) {
 
 using namespace kfb;
 
-#define KFB_SSM_CONFIG(ns, NS, TQ, ...)              \
-  if (ns == 4) { constexpr int NS = 4, TQ = 16; __VA_ARGS__; } \
-  else { constexpr int NS = 8, TQ = 8; __VA_ARGS__; }
+// NS states a wave and tiles of TQ steps; V channels a vector, IT vectors a
+// thread: 4 to 8 waves hold a tile.
+#define KFB_SSM_VEC(v, V, IT, one, ...)                    \
+  if (v == 4) { constexpr int V = 4, IT = 1; __VA_ARGS__; } \
+  else { constexpr int V = 1, IT = one; __VA_ARGS__; }
+
+#define KFB_SSM_CONFIG(p, v, V, IT, NS, TQ, ...)                                                          \
+  switch (p.ns) {                                                                                         \
+    case 1: { constexpr int NS = 1, TQ = 16; KFB_SSM_VEC(v, V, IT, 4, __VA_ARGS__) break; }                \
+    case 2: { constexpr int NS = 2, TQ = 16; KFB_SSM_VEC(v, V, IT, 4, __VA_ARGS__) break; }                \
+    case 4: { constexpr int NS = 4, TQ = 16; KFB_SSM_VEC(v, V, IT, 4, __VA_ARGS__) break; }                \
+    default: { constexpr int NS = 8, TQ = 8; KFB_SSM_VEC(v, V, IT, 2, __VA_ARGS__) break; }                \
+  }
 
 KFB_API int kfb_ssm_max_states() { return 64; }
 
-// Floats of: the fp32 copy of B and C (what = 0), the saved states of a
-// training forward (1), the backward's workspace (2).
+// Floats of: the fp32 copy of B and C and the forward's chunk ends (what = 0),
+// the saved states of a training forward (1), the backward's workspace (2).
 KFB_API long kfb_ssm_floats(int what, int T, int B, int D, int N) {
-  const ssm::Plan p = ssm::plan(T, N);
+  const ssm::Plan p = ssm::plan(T, B, D, N);
+  const long state = (long)B * N * D, chunk = state + (long)B * D;
   switch (what) {
-    case 0: return (long)B * p.W * p.Tp * 2 * p.ns;
-    case 1: return (long)p.tiles * B * N * D;
-    case 2: return (long)ceil_div(D, 64) * T * B * 2 * N + (long)B * (N + 2) * D;
+    case 0: return (long)B * p.W * p.Tp * 2 * p.ns + (p.fc > 1 ? p.fc * chunk : 0);
+    case 1: return (long)p.tiles * state;
+    case 2: return (long)ceil_div(D, 64) * T * B * 2 * N + (long)B * p.bc * (N + 2) * D +
+                   (p.bc > 1 ? p.bc * chunk : 0);
     default: return -1;
   }
 }
 
-KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V, const void* x, long ldx, const void* delta,
+KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V_, const void* x, long ldx, const void* delta,
                                     long ldd, const void* z, long ldz, const void* bm, long ldb,
                                     const void* cm, long ldc, const float* A, const float* skip,
                                     const float* bias, const int* len, const float* h0, float* hT,
                                     float* hs, float* bc, void* y, int T, int B, int D, int N,
                                     int softplus, int reverse, hipStream_t stream) {
-  const ssm::Plan p = ssm::plan(T, N > 0 ? N : 1);
   ssm::Args a{};
   a.x = x; a.delta = delta; a.z = z; a.bm = bm; a.cm = cm;
   a.ldx = ldx; a.ldd = ldd; a.ldz = ldz; a.ldb = ldb; a.ldc = ldc;
   a.A = A; a.skip = skip; a.bias = bias; a.len = len; a.h0 = h0; a.hT = hT; a.hs = hs; a.bc = bc;
   a.y = y;
-  a.T = T; a.B = B; a.D = D; a.N = N; a.W = p.W; a.Tp = p.Tp;
-  a.softplus = softplus; a.reverse = reverse;
-  if (ssm::bad(a) || (V != 1 && V != 4)) return hipErrorInvalidValue;
-  const dim3 grid(ceil_div(D, 64), B);
-  KFB_DISPATCH_DTYPE(dtype, E, {
-    KFB_SSM_CONFIG(p.ns, NS, TQ, {
-      const long total = (long)B * p.W * p.Tp * 2 * NS;
-      hipLaunchKernelGGL((ssm::prep_k<E, NS>), dim3(ceil_div(total < (1l << 22) ? total : (1l << 22), 256)),
-                         dim3(256), 0, stream, a);
-      const size_t shm = (size_t)(2 + p.W) * TQ * 64 * sizeof(float);
-      if (V == 4)
-        hipLaunchKernelGGL((ssm::scan_fwd_k<E, 4, NS, TQ>), grid, dim3(p.W * 64), shm, stream, a);
-      else
-        hipLaunchKernelGGL((ssm::scan_fwd_k<E, 1, NS, TQ>), grid, dim3(p.W * 64), shm, stream, a);
-    });
-  });
+  a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse;
+  if (ssm::bad(a) || (V_ != 1 && V_ != 4)) return hipErrorInvalidValue;
+  const ssm::Plan p = ssm::plan(T, B, D, N);
+  a.W = p.W; a.Tp = p.Tp;
+  ssm::cut(a, p, p.fc);
+  a.ends = bc + (long)B * p.W * p.Tp * 2 * p.ns;
+  a.sums = a.ends + (long)p.fc * B * N * D;
+  KFB_DISPATCH_DTYPE(dtype, E, KFB_SSM_CONFIG(p, V_, V, IT, NS, TQ, {
+    const long total = (long)B * p.W * p.Tp * 2 * NS;
+    hipLaunchKernelGGL((ssm::prep_k<E, NS>), dim3(ceil_div(total < (1l << 22) ? total : (1l << 22), 256)),
+                       dim3(256), 0, stream, a);
+    const size_t shm = (size_t)(2 + p.W) * TQ * 64 * sizeof(float);
+    dim3 grid(ceil_div(D, 64), B, a.nchunk - 1);
+    if (grid.z)
+      hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, true>), grid, dim3(p.W * 64),
+                         2 * TQ * 64 * sizeof(float), stream, a);
+    grid.z = a.nchunk;
+    hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, false>), grid, dim3(p.W * 64), shm, stream, a);
+  }));
   return hipGetLastError();
 }
 
-KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V, const void* dy, long ldy, const void* x,
+KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V_, const void* dy, long ldy, const void* x,
                                     long ldx, const void* delta, long ldd, const void* z, long ldz,
                                     const float* A, const float* skip, const float* bias,
                                     const int* len, const float* hs, float* bc, const float* dhT,
@@ -493,34 +751,39 @@ KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V, const void* dy, long ldy, 
                                     void* dc, float* dA, float* dskip, float* dbias, int acc_a,
                                     int acc_skip, int acc_bias, float* ws, int T, int B, int D,
                                     int N, int softplus, int reverse, hipStream_t stream) {
-  const ssm::Plan p = ssm::plan(T, N > 0 ? N : 1);
   ssm::Args a{};
   a.x = x; a.delta = delta; a.z = z; a.dy = dy;
   a.ldx = ldx; a.ldd = ldd; a.ldz = ldz; a.ldy = ldy;
   a.A = A; a.skip = skip; a.bias = bias; a.len = len; a.hs = const_cast<float*>(hs); a.bc = bc;
   a.dhT = dhT; a.dh0 = dh0; a.dx = dx; a.ddelta = ddelta; a.dz = dz;
-  a.T = T; a.B = B; a.D = D; a.N = N; a.W = p.W; a.Tp = p.Tp;
-  a.softplus = softplus; a.reverse = reverse;
-  if (ssm::bad(a) || (V != 1 && V != 4) || !ws || !hs) return hipErrorInvalidValue;
+  a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse;
+  if (ssm::bad(a) || (V_ != 1 && V_ != 4) || !ws || !hs) return hipErrorInvalidValue;
+  const ssm::Plan p = ssm::plan(T, B, D, N);
+  a.W = p.W; a.Tp = p.Tp;
+  ssm::cut(a, p, p.bc);
   const int nblk = ceil_div(D, 64);
   const long rows = (long)T * B;
   a.pbc = ws;
   a.pch = ws + (long)nblk * rows * 2 * N;
-  const dim3 grid(nblk, B);
+  a.ends = a.pch + (long)B * p.bc * (N + 2) * D;
+  a.sums = a.ends + (long)p.bc * B * N * D;
   KFB_DISPATCH_DTYPE(dtype, E, {
-    KFB_SSM_CONFIG(p.ns, NS, TQ, {
-      size_t shm = (size_t)(3 + 3 * p.W) * TQ * 64 * sizeof(float);
-      if (shm < (size_t)2 * 64 * p.W * V * sizeof(float)) shm = (size_t)2 * 64 * p.W * V * sizeof(float);
-      if (V == 4)
-        hipLaunchKernelGGL((ssm::scan_bwd_k<E, 4, NS, TQ>), grid, dim3(p.W * 64), shm, stream, a);
-      else
-        hipLaunchKernelGGL((ssm::scan_bwd_k<E, 1, NS, TQ>), grid, dim3(p.W * 64), shm, stream, a);
+    KFB_SSM_CONFIG(p, V_, V, IT, NS, TQ, {
+      size_t shm = sizeof(float) * ((size_t)(3 + 3 * p.W) * TQ * 64 + (size_t)TQ * 2 * p.W * NS);
+      const size_t last = sizeof(float) * 2 * 64 * p.W * V;
+      if (shm < last) shm = last;
+      dim3 grid(nblk, B, a.nchunk - 1);
+      if (grid.z)
+        hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, true>), grid, dim3(p.W * 64),
+                           3 * TQ * 64 * sizeof(float), stream, a);
+      grid.z = a.nchunk;
+      hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, false>), grid, dim3(p.W * 64), shm, stream, a);
     });
     hipLaunchKernelGGL((ssm::bc_grad_k<E>), dim3(ceil_div(rows * 2 * N < (1l << 22) ? rows * 2 * N : (1l << 22), 256)),
                        dim3(256), 0, stream, a.pbc, nblk, rows, N, (E*)db, (E*)dc);
   });
-  hipLaunchKernelGGL(ssm::param_grad_k, dim3(ceil_div((long)(N + 2) * D, 256)), dim3(256), 0, stream,
-                     a.pch, B, N, D, dA, dskip, dbias, acc_a, acc_skip, acc_bias);
+  hipLaunchKernelGGL(ssm::param_grad_k, dim3(ceil_div((long)(N + 2) * D, 32)), dim3(256), 0, stream,
+                     a.pch, B * a.nchunk, N, D, dA, dskip, dbias, acc_a, acc_skip, acc_bias);
   return hipGetLastError();
 }
 
