@@ -17,8 +17,8 @@ __device__ __forceinline__ float sigmoidf(float u) {
 }
 
 // u * sigmoid(u): below about -88 the exponential is infinite and u * 0 = -0,
-// but -inf * 0 would be NaN: the limit is 0.
-__device__ __forceinline__ float siluf(float u) { return u == -INFINITY ? 0.f : u * sigmoidf(u); }
+// but -inf * 0 would be NaN: the limit is 0.  (NaN comes through the sigmoid.)
+__device__ __forceinline__ float siluf(float u) { return fmaxf(u, -3.4e38f) * sigmoidf(u); }
 
 __device__ __forceinline__ float dsiluf(float u) {
   const float s = sigmoidf(u);
@@ -83,22 +83,18 @@ template <int KIND> __device__ __forceinline__ float act_grad(float u, const Act
     default: { constexpr int KIND = kfb::CLAMP; __VA_ARGS__; break; }  \
   }
 
-// e^v to about 1.5 ulp for any v: the rounding error of log2(e) v, kept from
-// the fused multiply-add, comes back as a first-order factor.
-__device__ __forceinline__ float exp_f(float v) {
-  const float p = LOG2E * v, lo = fmaf(LOG2E, v, -p) + 1.9259629911e-8f * v;
-  const float e = __builtin_amdgcn_exp2f(p);
-  return fabsf(p) < 126.f ? fmaf(e, LN2 * lo, e) : e;
-}
-
-// log(1 + e^v) = max(v, 0) + log1p(e^-|v|).  log1p(e) = log(w) e / (w - 1) with
-// w = 1 + e rounded (w - 1 is exact): the relative error stays at a few ulp for
-// small e, where log(w) alone loses what the rounding of w drops.
+// log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v|, to a few ulp for any v.
+// The rounding error of log2(e) |v|, kept from the fused multiply-add, comes back
+// as a first-order factor of e.  With w = 1 + e rounded and c = e - (w - 1), both
+// exact, log1p(e) = log(w) + c / w, and c alone is as good: it counts where w is
+// near 1 (for small e log(w) loses what the rounding of w drops).
 __device__ __forceinline__ float softplusf(float v) {
-  const float e = exp_f(-fabsf(v));
+  const float m = fmaxf(-fabsf(v), -200.f);  // e^-200 is 0 either way
+  const float p = LOG2E * m, lo = fmaf(LOG2E, m, -p);
+  float e = __builtin_amdgcn_exp2f(p);
+  e = fmaf(e, LN2 * lo, e);
   const float w = 1.f + e;
-  const float l = w == 1.f ? e : LN2 * __builtin_amdgcn_logf(w) * e * __builtin_amdgcn_rcpf(w - 1.f);
-  return fmaxf(v, 0.f) + (v != v ? v : l);
+  return fmaf(LN2, __builtin_amdgcn_logf(w), e - (w - 1.f)) + (v < 0.f ? 0.f : v);  // NaN stays
 }
 
 }  // namespace kfb

@@ -53,14 +53,25 @@ struct Args {
 // B and C as constant memory: uniform addresses become scalar loads
 typedef const __attribute__((address_space(4))) float cfloat;
 
-// The same address as a value the compiler does not know: loads through it are
-// neither merged with earlier ones nor moved up, which would keep more values
-// of B and C alive than there are scalar registers.
-__device__ __forceinline__ cfloat* fresh(const float* p) {
-  uintptr_t q = (uintptr_t)p;
-  asm volatile("" : "+s"(q));
-  return (cfloat*)q;
-}
+// B and C of UR steps for NS states, in scalar registers.  load() is given an
+// address that the compiler does not know to be an earlier one: the loads are
+// neither merged with others nor moved, so that a group is in flight while the one
+// before it is worked on and no more than two are alive (64 of the 102 registers).
+template <int NS, int UR> struct Group {
+  float v[UR * 2 * NS];
+  __device__ __forceinline__ void load(const float* p) {
+    uintptr_t q = (uintptr_t)p;
+    asm volatile("" : "+s"(q));
+    cfloat* c = (cfloat*)q;
+#pragma unroll
+    for (int i = 0; i < UR * 2 * NS; ++i) v[i] = c[i];
+    __builtin_amdgcn_sched_barrier(0x7ff);  // everything but scalar loads may pass
+  }
+  __device__ __forceinline__ float B(int k, int i) const { return v[k * 2 * NS + i]; }
+  __device__ __forceinline__ float C(int k, int i) const { return v[k * 2 * NS + NS + i]; }
+};
+
+constexpr int BC_PAD = 64;  // floats behind bc: a group is fetched ahead
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.T) : a.T;
@@ -110,28 +121,30 @@ template <typename T, int V, int IT, int TQ> struct Part {
       r[i] = q < TQ ? q : TQ;
     }
   }
-  // rows s0 + r of p (step elements apart, from position 0), zero past ``n``
-  __device__ __forceinline__ void load(const T* p, long step, int s0, int n, Raw<T, V> (&v)[IT]) const {
-#pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      if (on && r[i] < TQ && s0 + r[i] < n) v[i].load(p + (s0 + r[i]) * step + cl);
-      else v[i].zero();
-    }
-  }
 };
 
-// Position 0 of sequence b in a [T][B] tensor and the elements to the next.
-template <typename T>
-__device__ __forceinline__ const T* line(const Args& a, const void* p, long ld, int b, int d0,
-                                         int len, long& step) {
-  step = (long)a.B * ld;
-  const T* q = (const T*)p + (long)b * ld + d0;
-  if (a.reverse && len > 0) {
-    q += (len - 1) * step;
-    step = -step;
+// One sequence's rows of a [T][B] tensor: position s at p + s * step.  Loads are
+// unconditional: a position or channel outside reads the last one inside (of an
+// empty sequence: row 0), and what it gives is not used.
+template <typename T, int V> struct Line {
+  const T* p;
+  long step;
+  int last;
+
+  __device__ __forceinline__ Line(const Args& a, const void* t, long ld, int b, int c, int len) {
+    step = (long)a.B * ld;
+    p = (const T*)t + (long)b * ld + (c < a.D ? c : a.D - V);
+    last = len > 0 ? len - 1 : 0;
+    if (a.reverse && len > 0) {
+      p += last * step;
+      step = -step;
+    }
   }
-  return q;
-}
+  template <int IT> __device__ __forceinline__ void load(const int (&r)[IT], int s0, Raw<T, V> (&v)[IT]) const {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) v[i].load(p + min(s0 + r[i], last) * step);
+  }
+};
 
 template <int V>
 __device__ __forceinline__ void params(const float* p, int c, bool on, float (&v)[V]) {
@@ -143,126 +156,156 @@ __device__ __forceinline__ float step_size(float raw, bool softplus) {
   return softplus ? softplusf(raw) : raw;
 }
 
+// h over ``n`` chunks j = from, from + by, ...: h = exp(A sum dt_j) h + end_j,
+// eight chunks' values in flight.
+template <int NS>
+__device__ __forceinline__ void join(const Args& a, int b, int dc, long bnd, long bn, int ns,
+                                     const float (&A2)[NS], int from, int by, int n, float (&h)[NS]) {
+  constexpr int Q = NS > 4 ? 4 : 8;
+  for (int j0 = 0; j0 < n; j0 += Q) {
+    float sum[Q], end[Q][NS];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int j = from + by * min(j0 + q, n - 1);
+      sum[q] = a.sums[((long)j * a.B + b) * a.D + dc];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) end[q][i] = i < ns ? a.ends[j * bn + bnd + (long)i * a.D] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (j0 + q < n)
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          if (i < ns) h[i] = fmaf(__builtin_amdgcn_exp2f(sum[q] * A2[i]), h[i], end[q][i]);
+  }
+}
+
+// The order in a tile is for the memory counter, which counts loads and stores in
+// turn: the next tile's rows are fetched before the walk and used before y is stored,
+// so that no wait for a load waits for a store just issued.
 // ENDS: only the state after each chunk, from zero, and the chunk's sum of dt.
 template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   extern __shared__ float lds[];
-  constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;  // steps whose B and C are in scalar registers
+  constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;  // steps of a group
   float2* du = (float2*)lds;           // [TQ][64]
   float* yp = lds + TQ * 64 * 2;       // [W][TQ][64]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane, chunk = blockIdx.z;
-  const int len = seq_len(a, b);
-  const long bnd = ((long)b * a.N + w * NS) * a.D + d, bn = (long)a.B * a.N * a.D;
+  const int len = seq_len(a, b), ns = min(max(a.N - w * NS, 0), NS);  // states of this wave
+  const bool ok = d < a.D;
+  const int dc = ok ? d : a.D - 1;
+  const long bnd = ((long)b * a.N + w * NS) * a.D + dc, bn = (long)a.B * a.N * a.D;
   float A2[NS], h[NS];
-  bool on[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    on[i] = w * NS + i < a.N && d < a.D;
-    A2[i] = on[i] ? a.A[(long)(w * NS + i) * a.D + d] * LOG2E : 0.f;
-    h[i] = on[i] && a.h0 && !ENDS ? a.h0[bnd + (long)i * a.D] : 0.f;
+    A2[i] = i < ns ? a.A[(long)(w * NS + i) * a.D + dc] * LOG2E : 0.f;
+    h[i] = i < ns && a.h0 && !ENDS ? a.h0[bnd + (long)i * a.D] : 0.f;
   }
-  if constexpr (!ENDS)
-    for (int j = 0; j < chunk; ++j) {
-      const float sum = d < a.D ? a.sums[((long)j * a.B + b) * a.D + d] : 0.f;
-#pragma unroll
-      for (int i = 0; i < NS; ++i)
-        if (on[i])
-          h[i] = fmaf(__builtin_amdgcn_exp2f(sum * A2[i]), h[i], a.ends[j * bn + bnd + (long)i * a.D]);
-    }
+  if constexpr (!ENDS) join<NS>(a, b, dc, bnd, bn, ns, A2, 0, 1, chunk, h);
   const float* bcw = a.bc + ((long)b * a.W + w) * a.Tp * 2 * NS;
   const Part<T, V, IT, TQ> me(a, d0);
-  long stx, std, stz = 0;
-  const T* px = line<T>(a, a.x, a.ldx, b, d0, len, stx);
-  const T* pd = line<T>(a, a.delta, a.ldd, b, d0, len, std);
-  const T* pz = a.z ? line<T>(a, a.z, a.ldz, b, d0, len, stz) : px;
+  const Line<T, V> lx(a, a.x, a.ldx, b, me.c, len), ld(a, a.delta, a.ldd, b, me.c, len);
+  const bool gate = !ENDS && a.z;
+  const Line<T, V> lz(a, gate ? a.z : a.x, gate ? a.ldz : a.ldx, b, me.c, len);
   float bias[V], skip[V];
   params<V>(a.bias, me.c, me.on, bias);
   params<V>(a.skip, me.c, me.on, skip);
   Raw<T, V> nx[IT], nd[IT], nz[IT], cx[IT], cz[IT];
   const int s_end = min((chunk + 1) * a.tpc * TQ, a.Tp);
   auto fetch = [&](int s0) {
-    me.load(px, stx, s0, len, nx);
-    me.load(pd, std, s0, len, nd);
-    if (!ENDS && a.z) me.load(pz, stz, s0, len, nz);
+    lx.load(me.r, s0, nx);
+    ld.load(me.r, s0, nd);
+    if (!ENDS) lz.load(me.r, s0, nz);
   };
   auto stage = [&](int s0) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
+    for (int i = 0; i < IT; ++i)
       if (me.r[i] < TQ) {
         const bool in = me.on && s0 + me.r[i] < len;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float dt = in ? step_size(nd[i][k] + bias[k], a.softplus) : 0.f;
-          du[me.r[i] * 64 + me.cl + k] = make_float2(dt, dt * nx[i][k]);
+          const float dt = step_size(nd[i][k] + bias[k], a.softplus);
+          du[me.r[i] * 64 + me.cl + k] = make_float2(in ? dt : 0.f, in ? dt * nx[i][k] : 0.f);
         }
       }
-      cx[i] = nx[i];
-      cz[i] = nz[i];
-    }
   };
   float sum_dt = 0.f;
   int s0 = chunk * a.tpc * TQ;
+  Group<NS, UR> next;
+  next.load(bcw + (long)s0 * 2 * NS);
   fetch(s0);
   stage(s0);
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    cx[i] = nx[i];
+    cz[i] = nz[i];
+  }
   __syncthreads();
   for (; s0 < s_end; s0 += TQ) {
     const bool more = s0 + TQ < s_end;
-    if (more) fetch(s0 + TQ);
-    if (!ENDS && a.hs) {
+    fetch(more ? s0 + TQ : s0);
+    if (!ENDS && a.hs && ok) {
       float* hs = a.hs + (long)(s0 / TQ) * bn + bnd;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
-        if (on[i]) hs[(long)i * a.D] = h[i];
+        if (i < ns) hs[(long)i * a.D] = h[i];
     }
 #pragma unroll
     for (int r0 = 0; r0 < TQ; r0 += UR) {
-      cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+      const Group<NS, UR> bc = next;
+      next.load(bcw + (long)(s0 + r0 + UR) * 2 * NS);
 #pragma unroll
       for (int k = 0; k < UR; ++k) {
         const float2 u = du[(r0 + k) * 64 + lane];
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          h[i] = fmaf(__builtin_amdgcn_exp2f(u.x * A2[i]), h[i], u.y * bct[k * 2 * NS + i]);
-          if (!ENDS) v = fmaf(bct[k * 2 * NS + NS + i], h[i], v);
+          h[i] = fmaf(__builtin_amdgcn_exp2f(u.x * A2[i]), h[i], u.y * bc.B(k, i));
+          if (!ENDS) v = fmaf(bc.C(k, i), h[i], v);
         }
         if constexpr (ENDS) sum_dt += u.x;
         else yp[(w * TQ + r0 + k) * 64 + lane] = v;
       }
     }
     __syncthreads();
+    if (more) stage(s0 + TQ);
     if constexpr (!ENDS) {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         const int r = me.r[i], s = s0 + r;
-        if (r >= TQ || s >= a.T || !me.on) continue;
-        float v[V];
+        if (r < TQ) {
+          float v[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = skip[k] * cx[i][k];
-        for (int q = 0; q < a.W; ++q)
+          for (int k = 0; k < V; ++k) v[k] = skip[k] * cx[i][k];
 #pragma unroll
-          for (int k = 0; k < V; ++k) v[k] += yp[(q * TQ + r) * 64 + me.cl + k];
-        if (a.z)
+          for (int q = 0; q < 8; ++q)
+            if (q < a.W)
 #pragma unroll
-          for (int k = 0; k < V; ++k) v[k] *= siluf(cz[i][k]);
+              for (int k = 0; k < V; ++k) v[k] += yp[(q * TQ + r) * 64 + me.cl + k];
+          if (gate)
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = s < len ? v[k] : 0.f;
-        store_vec<T, V>((T*)a.y + row_of(a, b, s, len) * a.D + me.c, v);
+            for (int k = 0; k < V; ++k) v[k] *= siluf(cz[i][k]);
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] = s < len ? v[k] : 0.f;
+          if (s < a.T && me.on) store_vec<T, V>((T*)a.y + row_of(a, b, s, len) * a.D + me.c, v);
+        }
+        cx[i] = nx[i];
+        cz[i] = nz[i];
       }
     }
-    if (more) stage(s0 + TQ);
     __syncthreads();
   }
   if constexpr (ENDS) {
+    if (ok)
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (i < ns) a.ends[chunk * bn + bnd + (long)i * a.D] = h[i];
+    if (w == 0 && ok) a.sums[((long)chunk * a.B + b) * a.D + d] = sum_dt;
+  } else if (a.hT && chunk == a.nchunk - 1 && ok) {
 #pragma unroll
     for (int i = 0; i < NS; ++i)
-      if (on[i]) a.ends[chunk * bn + bnd + (long)i * a.D] = h[i];
-    if (w == 0 && d < a.D) a.sums[((long)chunk * a.B + b) * a.D + d] = sum_dt;
-  } else if (a.hT && chunk == a.nchunk - 1) {
-#pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (on[i]) a.hT[bnd + (long)i * a.D] = h[i];
+      if (i < ns) a.hT[bnd + (long)i * a.D] = h[i];
   }
 }
 
@@ -332,53 +375,54 @@ template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   extern __shared__ float lds[];
   const int WN = a.W * NS;
-  constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;
+  constexpr int UR = 8 / NS < 4 ? 8 / NS : 4;
   float2* du = (float2*)lds;                    // [TQ][64] dt, dt x
   float* se = lds + TQ * 64 * 2;                // [TQ][64] e
   float* sbc = se + TQ * 64;                    // [TQ][2 WN]
-  float* yp = sbc + TQ * 2 * WN;                // [W][TQ][64]
+  float* yp = sbc + TQ * 2 * WN + 64;           // [W][TQ][64]
   float2* pq = (float2*)(yp + a.W * TQ * 64);   // [W][TQ][64]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane;
   const int chunk = ENDS ? blockIdx.z + 1 : blockIdx.z;
-  const int len = seq_len(a, b), nt = a.W * 64;
-  const long bnd = ((long)b * a.N + w * NS) * a.D + d, bn = (long)a.B * a.N * a.D;
+  const int len = seq_len(a, b), nt = a.W * 64, ns = min(max(a.N - w * NS, 0), NS);
+  const bool ok = d < a.D;
+  const int dc = ok ? d : a.D - 1;
+  const long bnd = ((long)b * a.N + w * NS) * a.D + dc, bn = (long)a.B * a.N * a.D;
   float A1[NS], carry[NS], dA[NS];
-  bool on[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    on[i] = w * NS + i < a.N && d < a.D;
-    A1[i] = on[i] ? a.A[(long)(w * NS + i) * a.D + d] : 0.f;
-    carry[i] = on[i] && a.dhT && !ENDS ? a.dhT[bnd + (long)i * a.D] : 0.f;
+    A1[i] = i < ns && ok ? a.A[(long)(w * NS + i) * a.D + dc] : 0.f;
+    carry[i] = i < ns && ok && a.dhT && !ENDS ? a.dhT[bnd + (long)i * a.D] : 0.f;
     dA[i] = 0.f;
   }
-  if constexpr (!ENDS)
-    for (int j = a.nchunk - 1; j > chunk; --j) {
-      const float sum = d < a.D ? a.sums[((long)j * a.B + b) * a.D + d] : 0.f;
+  if constexpr (!ENDS) {
+    float A2[NS];
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
-        if (on[i])
-          carry[i] = fmaf(__builtin_amdgcn_exp2f(sum * (A1[i] * LOG2E)), carry[i],
-                          a.ends[j * bn + bnd + (long)i * a.D]);
-    }
+    for (int i = 0; i < NS; ++i) A2[i] = A1[i] * LOG2E;
+    join<NS>(a, b, dc, bnd, bn, ok ? ns : 0, A2, a.nchunk - 1, -1, a.nchunk - 1 - chunk, carry);
+  }
   const float* bcw = a.bc + ((long)b * a.W + w) * a.Tp * 2 * NS;
   const Part<T, V, IT, TQ> me(a, d0);
-  long stx, std, sty, stz = 0;
-  const T* px = line<T>(a, a.x, a.ldx, b, d0, len, stx);
-  const T* pd = line<T>(a, a.delta, a.ldd, b, d0, len, std);
-  const T* py = line<T>(a, a.dy, a.ldy, b, d0, len, sty);
-  const T* pz = a.z ? line<T>(a, a.z, a.ldz, b, d0, len, stz) : px;
+  const bool gate = a.z;
+  const Line<T, V> lx(a, a.x, a.ldx, b, me.c, len), ld(a, a.delta, a.ldd, b, me.c, len),
+      ly(a, a.dy, a.ldy, b, me.c, len), lz(a, gate ? a.z : a.x, gate ? a.ldz : a.ldx, b, me.c, len);
   float bias[V], skip[V], gskip[V], gbias[V];
   params<V>(a.bias, me.c, me.on, bias);
   params<V>(a.skip, me.c, me.on, skip);
 #pragma unroll
   for (int k = 0; k < V; ++k) gskip[k] = gbias[k] = 0.f;
   Raw<T, V> nx[IT], nd[IT], ny[IT], nz[IT], cx[IT], cd[IT], cy[IT], cz[IT];
+  float hb[NS], hn[NS];  // the state before this tile and before the next one
   auto fetch = [&](int s0) {
-    if (!ENDS) me.load(px, stx, s0, len, nx);
-    me.load(pd, std, s0, len, nd);
-    me.load(py, sty, s0, len, ny);
-    if (a.z) me.load(pz, stz, s0, len, nz);
+    if (!ENDS) lx.load(me.r, s0, nx);
+    ld.load(me.r, s0, nd);
+    ly.load(me.r, s0, ny);
+    lz.load(me.r, s0, nz);
+    if (!ENDS) {
+      const float* hs = a.hs + (long)(s0 / TQ) * bn + bnd;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) hn[i] = hs[i < ns ? (long)i * a.D : 0];
+    }
   };
   auto stage = [&](int s0) {
 #pragma unroll
@@ -387,9 +431,10 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
         const bool in = me.on && s0 + me.r[i] < len;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float dt = in ? step_size(nd[i][k] + bias[k], a.softplus) : 0.f;
-          du[me.r[i] * 64 + me.cl + k] = make_float2(dt, ENDS ? 0.f : dt * nx[i][k]);
-          se[me.r[i] * 64 + me.cl + k] = a.z ? ny[i][k] * siluf(nz[i][k]) : ny[i][k];
+          const float dt = step_size(nd[i][k] + bias[k], a.softplus);
+          const float e = gate ? ny[i][k] * siluf(nz[i][k]) : ny[i][k];
+          du[me.r[i] * 64 + me.cl + k] = make_float2(in ? dt : 0.f, in && !ENDS ? dt * nx[i][k] : 0.f);
+          se[me.r[i] * 64 + me.cl + k] = in ? e : 0.f;
         }
       }
       cx[i] = nx[i];
@@ -397,45 +442,50 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
       cy[i] = ny[i];
       cz[i] = nz[i];
     }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) hb[i] = i < ns && ok ? hn[i] : 0.f;
   };
-  // where a lane's sum of lanes_sum goes in a row of sbc
+  // where a lane's sum of lanes_sum goes in a row of sbc; a lane whose sum is
+  // another lane's too writes behind the rows (no branch in the walk)
   const int val = lane_value<2 * NS>(lane);
-  const int col = val < NS ? w * NS + val : WN + w * NS + val - NS;
   const bool writer = (lane & (32 / NS - 1)) == 0;
+  const int col = !writer ? TQ * 2 * WN + lane : val < NS ? w * NS + val : WN + w * NS + val - NS;
+  const int row = writer ? 2 * WN : 0;
   const int t0 = chunk * a.tpc, t1 = min(t0 + a.tpc, a.Tp / TQ);
   float sum_dt = 0.f;
+  Group<NS, UR> next;
+  next.load(bcw + (long)(ENDS ? t1 * TQ - UR : (t1 - 1) * TQ) * 2 * NS);
   fetch((t1 - 1) * TQ);
   stage((t1 - 1) * TQ);
   __syncthreads();
   for (int tile = t1 - 1; tile >= t0; --tile) {
     const int s0 = tile * TQ;
-    if (tile > t0) fetch(s0 - TQ);
+    const bool more = tile > t0;
     if constexpr (ENDS) {
+      fetch(more ? s0 - TQ : s0);
 #pragma unroll
       for (int r0 = TQ - UR; r0 >= 0; r0 -= UR) {
-        cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+        const Group<NS, UR> bc = next;
+        next.load(bcw + (long)max(s0 + r0 - UR, 0) * 2 * NS);
 #pragma unroll
         for (int k = UR - 1; k >= 0; --k) {
           const float dt = du[(r0 + k) * 64 + lane].x, e = se[(r0 + k) * 64 + lane];
           sum_dt += dt;
 #pragma unroll
           for (int i = 0; i < NS; ++i)
-            carry[i] = fmaf(bct[k * 2 * NS + NS + i], e, carry[i]) *
-                       __builtin_amdgcn_exp2f(dt * (A1[i] * LOG2E));
+            carry[i] = fmaf(bc.C(k, i), e, carry[i]) * __builtin_amdgcn_exp2f(dt * (A1[i] * LOG2E));
         }
       }
       __syncthreads();
+      if (more) stage(s0 - TQ);
     } else {
-      float hb[NS], H[TQ][NS], dec[TQ][NS], dAt[NS];
-      const float* hs = a.hs + (long)tile * bn + bnd;
+      float H[TQ][NS], dec[TQ][NS], dAt[NS];
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        hb[i] = on[i] ? hs[(long)i * a.D] : 0.f;
-        dAt[i] = 0.f;
-      }
+      for (int i = 0; i < NS; ++i) dAt[i] = 0.f;
 #pragma unroll
       for (int r0 = 0; r0 < TQ; r0 += UR) {
-        cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+        const Group<NS, UR> bc = next;
+        if (r0 + UR < TQ) next.load(bcw + (long)(s0 + r0 + UR) * 2 * NS);
 #pragma unroll
         for (int k = 0; k < UR; ++k) {
           const int r = r0 + k;
@@ -444,15 +494,17 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
             dec[r][i] = __builtin_amdgcn_exp2f(u.x * (A1[i] * LOG2E));
-            H[r][i] = fmaf(dec[r][i], r ? H[r - 1][i] : hb[i], u.y * bct[k * 2 * NS + i]);
-            v = fmaf(bct[k * 2 * NS + NS + i], H[r][i], v);
+            H[r][i] = fmaf(dec[r][i], r ? H[r - 1][i] : hb[i], u.y * bc.B(k, i));
+            v = fmaf(bc.C(k, i), H[r][i], v);
           }
-          if (a.z) yp[(w * TQ + r) * 64 + lane] = v;
+          yp[(w * TQ + r) * 64 + lane] = v;
         }
       }
 #pragma unroll
       for (int r0 = TQ - UR; r0 >= 0; r0 -= UR) {
-        cfloat* bct = fresh(bcw + (long)(s0 + r0) * 2 * NS);
+        const Group<NS, UR> bc = next;
+        // the group before; behind a tile's first one comes the earlier tile's first
+        next.load(bcw + (long)max(r0 ? s0 + r0 - UR : s0 - TQ, 0) * 2 * NS);
 #pragma unroll
         for (int k = UR - 1; k >= 0; --k) {
           const int r = r0 + k;
@@ -461,8 +513,8 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
           float p = 0.f, q = 0.f, red[2 * NS];
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
-            const float g = fmaf(bct[k * 2 * NS + NS + i], e, carry[i]);
-            p = fmaf(g, bct[k * 2 * NS + i], p);
+            const float g = fmaf(bc.C(k, i), e, carry[i]);
+            p = fmaf(g, bc.B(k, i), p);
             red[i] = g * u.y;
             red[NS + i] = e * H[r][i];
             carry[i] = g * dec[r][i];
@@ -472,80 +524,90 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
           }
           pq[(w * TQ + r) * 64 + lane] = make_float2(p, q);
           const float s = lanes_sum<2 * NS>(red, lane);
-          if (writer) sbc[r * 2 * WN + col] = s;
+          sbc[col + r * row] = s;
         }
       }
+      fetch(more ? s0 - TQ : s0);  // here, where H and dec have left their registers
 #pragma unroll
       for (int i = 0; i < NS; ++i) dA[i] += dAt[i];
       __syncthreads();
+      float ox[IT][V], od[IT][V], oz[IT][V];
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int r = me.r[i];
+        if (r >= TQ) continue;
+        const bool in = s0 + r < len;
+        float p[V], q[V], v[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) p[k] = q[k] = v[k] = 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (u < a.W)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+              const float2 t = pq[(u * TQ + r) * 64 + me.cl + k];
+              p[k] += t.x;
+              q[k] += t.y;
+              if (gate) v[k] += yp[(u * TQ + r) * 64 + me.cl + k];
+            }
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float x = in ? cx[i][k] : 0.f, e = se[r * 64 + me.cl + k], dt = du[r * 64 + me.cl + k].x;
+          float dd = fmaf(x, p[k], q[k]);
+          if (a.softplus) dd *= sigmoidf(cd[i][k] + bias[k]);
+          ox[i][k] = in ? fmaf(dt, p[k], skip[k] * e) : 0.f;
+          od[i][k] = in ? dd : 0.f;
+          oz[i][k] = in && gate ? cy[i][k] * fmaf(skip[k], x, v[k]) * dsiluf(cz[i][k]) : 0.f;
+          gskip[k] = fmaf(e, x, gskip[k]);
+          gbias[k] += od[i][k];
+        }
+      }
+      // (a thread stages the elements that it has just read)
+      if (more) stage(s0 - TQ);
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int s = s0 + me.r[i];
+        if (me.r[i] < TQ && s < a.T && me.on) {
+          const long at = row_of(a, b, s, len) * a.D + me.c;
+          store_vec<T, V>((T*)a.dx + at, ox[i]);
+          store_vec<T, V>((T*)a.ddelta + at, od[i]);
+          if (gate) store_vec<T, V>((T*)a.dz + at, oz[i]);
+        }
+      }
       for (int i = threadIdx.x; i < TQ * 2 * a.N; i += nt) {
         const int r = i / (2 * a.N), j = i - r * 2 * a.N, s = s0 + r;
         if (s < a.T)
           a.pbc[((long)blockIdx.x * a.T * a.B + row_of(a, b, s, len)) * 2 * a.N + j] =
               sbc[r * 2 * WN + (j < a.N ? j : WN + j - a.N)];
       }
-#pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const int r = me.r[i], s = s0 + r;
-        if (r >= TQ || s >= a.T || !me.on) continue;
-        float ox[V], od[V], oz[V];
-        const bool in = s < len;
-        float p[V], q[V], v[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) p[k] = q[k] = v[k] = 0.f;
-        for (int u = 0; u < a.W; ++u)
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const float2 t = pq[(u * TQ + r) * 64 + me.cl + k];
-            p[k] += t.x;
-            q[k] += t.y;
-            if (a.z) v[k] += yp[(u * TQ + r) * 64 + me.cl + k];
-          }
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float x = cx[i][k], e = se[r * 64 + me.cl + k], dt = du[r * 64 + me.cl + k].x;
-          float dd = fmaf(x, p[k], q[k]);
-          if (a.softplus) dd *= sigmoidf(cd[i][k] + bias[k]);
-          ox[k] = in ? fmaf(dt, p[k], skip[k] * e) : 0.f;
-          od[k] = in ? dd : 0.f;
-          oz[k] = in && a.z ? cy[i][k] * fmaf(skip[k], x, v[k]) * dsiluf(cz[i][k]) : 0.f;
-          gskip[k] = fmaf(e, x, gskip[k]);
-          gbias[k] += od[k];
-        }
-        const long at = row_of(a, b, s, len) * a.D + me.c;
-        store_vec<T, V>((T*)a.dx + at, ox);
-        store_vec<T, V>((T*)a.ddelta + at, od);
-        if (a.z) store_vec<T, V>((T*)a.dz + at, oz);
-      }
-      __syncthreads();
     }
-    if (tile > t0) stage(s0 - TQ);
     __syncthreads();
   }
   if constexpr (ENDS) {
+    if (ok)
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
-      if (on[i]) a.ends[chunk * bn + bnd + (long)i * a.D] = carry[i];
-    if (w == 0 && d < a.D) a.sums[((long)chunk * a.B + b) * a.D + d] = sum_dt;
+      for (int i = 0; i < NS; ++i)
+        if (i < ns) a.ends[chunk * bn + bnd + (long)i * a.D] = carry[i];
+    if (w == 0 && ok) a.sums[((long)chunk * a.B + b) * a.D + d] = sum_dt;
     return;
   }
   float* pch = a.pch + ((long)chunk * a.B + b) * (a.N + 2) * a.D;
+  if (ok)
 #pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    if (on[i]) {
-      pch[(long)(w * NS + i) * a.D + d] = dA[i];
-      if (a.dh0 && chunk == 0) a.dh0[bnd + (long)i * a.D] = carry[i];
-    }
-  }
+    for (int i = 0; i < NS; ++i)
+      if (i < ns) {
+        pch[(long)(w * NS + i) * a.D + d] = dA[i];
+        if (a.dh0 && chunk == 0) a.dh0[bnd + (long)i * a.D] = carry[i];
+      }
   // dskip, dbias: a thread holds V channels of some rows
-  const int nrow = nt / (64 / V), row = threadIdx.x / (64 / V);
+  const int nrow = nt / (64 / V), mine = threadIdx.x / (64 / V);
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    lds[row * 64 + me.cl + k] = gskip[k];
-    lds[(nrow + row) * 64 + me.cl + k] = gbias[k];
+    lds[mine * 64 + me.cl + k] = gskip[k];
+    lds[(nrow + mine) * 64 + me.cl + k] = gbias[k];
   }
   __syncthreads();
-  if (w == 0 && d < a.D) {
+  if (w == 0 && ok) {
     float u = 0.f, v = 0.f;
     for (int r = 0; r < nrow; ++r) {
       u += lds[r * 64 + lane];
@@ -659,7 +721,7 @@ inline Plan plan(int T, int B, int D, int N) {
   p.tiles = ceil_div(T, p.tq);
   p.Tp = p.tiles * p.tq;
   const long wgs = (long)ceil_div(D, 64) * B;
-  p.fc = chunks_of(wgs, p.tiles, 1024);
+  p.fc = chunks_of(wgs, p.tiles, 2048);
   p.bc = chunks_of(wgs, p.tiles, 512);
   return p;
 }
@@ -702,7 +764,7 @@ KFB_API long kfb_ssm_floats(int what, int T, int B, int D, int N) {
   const ssm::Plan p = ssm::plan(T, B, D, N);
   const long state = (long)B * N * D, chunk = state + (long)B * D;
   switch (what) {
-    case 0: return (long)B * p.W * p.Tp * 2 * p.ns + (p.fc > 1 ? p.fc * chunk : 0);
+    case 0: return (long)B * p.W * p.Tp * 2 * p.ns + ssm::BC_PAD + (p.fc > 1 ? p.fc * chunk : 0);
     case 1: return (long)p.tiles * state;
     case 2: return (long)ceil_div(D, 64) * T * B * 2 * N + (long)B * p.bc * (N + 2) * D +
                    (p.bc > 1 ? p.bc * chunk : 0);
@@ -726,7 +788,7 @@ KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V_, const void* x, long ldx, 
   const ssm::Plan p = ssm::plan(T, B, D, N);
   a.W = p.W; a.Tp = p.Tp;
   ssm::cut(a, p, p.fc);
-  a.ends = bc + (long)B * p.W * p.Tp * 2 * p.ns;
+  a.ends = bc + (long)B * p.W * p.Tp * 2 * p.ns + ssm::BC_PAD;
   a.sums = a.ends + (long)p.fc * B * N * D;
   KFB_DISPATCH_DTYPE(dtype, E, KFB_SSM_CONFIG(p, V_, V, IT, NS, TQ, {
     const long total = (long)B * p.W * p.Tp * 2 * NS;
@@ -769,7 +831,7 @@ KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V_, const void* dy, long ldy,
   a.sums = a.ends + (long)p.bc * B * N * D;
   KFB_DISPATCH_DTYPE(dtype, E, {
     KFB_SSM_CONFIG(p, V_, V, IT, NS, TQ, {
-      size_t shm = sizeof(float) * ((size_t)(3 + 3 * p.W) * TQ * 64 + (size_t)TQ * 2 * p.W * NS);
+      size_t shm = sizeof(float) * ((size_t)(3 + 3 * p.W) * TQ * 64 + (size_t)TQ * 2 * p.W * NS + 64);
       const size_t last = sizeof(float) * 2 * 64 * p.W * V;
       if (shm < last) shm = last;
       dim3 grid(nblk, B, a.nchunk - 1);
