@@ -153,7 +153,8 @@ __device__ __forceinline__ void params(const float* p, int c, bool on, float (&v
 }
 
 __device__ __forceinline__ float step_size(float raw, bool softplus) {
-  return softplus ? softplusf(raw) : raw;
+  const float v = softplusf(raw);  // (a select, not a branch: the flag is uniform)
+  return softplus ? v : raw;
 }
 
 // h over ``n`` chunks j = from, from + by, ...: h = exp(A sum dt_j) h + end_j,
@@ -188,8 +189,8 @@ template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   extern __shared__ float lds[];
   constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;  // steps of a group
-  float2* du = (float2*)lds;           // [TQ][64]
-  float* yp = lds + TQ * 64 * 2;       // [W][TQ][64]
+  float *sd = lds, *sx = lds + TQ * 64;  // [TQ][64] dt, dt x
+  float* yp = lds + TQ * 64 * 2;         // [W][TQ][64]
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane, chunk = blockIdx.z;
   const int len = seq_len(a, b), ns = min(max(a.N - w * NS, 0), NS);  // states of this wave
@@ -223,10 +224,12 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
     for (int i = 0; i < IT; ++i)
       if (me.r[i] < TQ) {
         const bool in = me.on && s0 + me.r[i] < len;
+        const int at = me.r[i] * 64 + me.cl;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const float dt = step_size(nd[i][k] + bias[k], a.softplus);
-          du[me.r[i] * 64 + me.cl + k] = make_float2(in ? dt : 0.f, in ? dt * nx[i][k] : 0.f);
+          sd[at + k] = in ? dt : 0.f;
+          sx[at + k] = in ? dt * nx[i][k] : 0.f;
         }
       }
   };
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
       next.load(bcw + (long)(s0 + r0 + UR) * 2 * NS);
 #pragma unroll
       for (int k = 0; k < UR; ++k) {
-        const float2 u = du[(r0 + k) * 64 + lane];
+        const float2 u = make_float2(sd[(r0 + k) * 64 + lane], sx[(r0 + k) * 64 + lane]);
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
@@ -278,11 +281,14 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
           float v[V];
 #pragma unroll
           for (int k = 0; k < V; ++k) v[k] = skip[k] * cx[i][k];
+          const float* part = yp + r * 64 + me.cl;
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q < a.W)
+          for (int q = 0; q < 4; ++q)  // W >= 4
 #pragma unroll
-              for (int k = 0; k < V; ++k) v[k] += yp[(q * TQ + r) * 64 + me.cl + k];
+            for (int k = 0; k < V; ++k) v[k] += part[q * TQ * 64 + k];
+          for (int q = 4; q < a.W; ++q)
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] += part[q * TQ * 64 + k];
           if (gate)
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] *= siluf(cz[i][k]);
@@ -376,11 +382,10 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   extern __shared__ float lds[];
   const int WN = a.W * NS;
   constexpr int UR = 8 / NS < 4 ? 8 / NS : 4;
-  float2* du = (float2*)lds;                    // [TQ][64] dt, dt x
-  float* se = lds + TQ * 64 * 2;                // [TQ][64] e
-  float* sbc = se + TQ * 64;                    // [TQ][2 WN]
-  float* yp = sbc + TQ * 2 * WN + 64;           // [W][TQ][64]
-  float2* pq = (float2*)(yp + a.W * TQ * 64);   // [W][TQ][64]
+  float *sd = lds, *sx = lds + TQ * 64, *se = lds + TQ * 64 * 2;  // [TQ][64] dt, dt x, e
+  float* sbc = se + TQ * 64;                                      // [TQ][2 WN] and a lane's rest
+  float* pp = sbc + TQ * 2 * WN + 64;                             // [W][TQ][64]: p, q, sum_n C h
+  float *pq = pp + a.W * TQ * 64, *yp = pq + a.W * TQ * 64;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int b = blockIdx.y, d0 = blockIdx.x * 64, d = d0 + lane;
   const int chunk = ENDS ? blockIdx.z + 1 : blockIdx.z;
@@ -429,12 +434,19 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
     for (int i = 0; i < IT; ++i) {
       if (me.r[i] < TQ) {
         const bool in = me.on && s0 + me.r[i] < len;
+        const int at = me.r[i] * 64 + me.cl;
+        float e[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) e[k] = ny[i][k];
+        if (gate)
+#pragma unroll
+          for (int k = 0; k < V; ++k) e[k] *= siluf(nz[i][k]);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const float dt = step_size(nd[i][k] + bias[k], a.softplus);
-          const float e = gate ? ny[i][k] * siluf(nz[i][k]) : ny[i][k];
-          du[me.r[i] * 64 + me.cl + k] = make_float2(in ? dt : 0.f, in && !ENDS ? dt * nx[i][k] : 0.f);
-          se[me.r[i] * 64 + me.cl + k] = in ? e : 0.f;
+          sd[at + k] = in ? dt : 0.f;
+          if (!ENDS) sx[at + k] = in ? dt * nx[i][k] : 0.f;
+          se[at + k] = in ? e[k] : 0.f;
         }
       }
       cx[i] = nx[i];
@@ -469,7 +481,7 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
         next.load(bcw + (long)max(s0 + r0 - UR, 0) * 2 * NS);
 #pragma unroll
         for (int k = UR - 1; k >= 0; --k) {
-          const float dt = du[(r0 + k) * 64 + lane].x, e = se[(r0 + k) * 64 + lane];
+          const float dt = sd[(r0 + k) * 64 + lane], e = se[(r0 + k) * 64 + lane];
           sum_dt += dt;
 #pragma unroll
           for (int i = 0; i < NS; ++i)
@@ -489,7 +501,7 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
 #pragma unroll
         for (int k = 0; k < UR; ++k) {
           const int r = r0 + k;
-          const float2 u = du[r * 64 + lane];
+          const float2 u = make_float2(sd[r * 64 + lane], sx[r * 64 + lane]);
           float v = 0.f;
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
@@ -508,7 +520,7 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
 #pragma unroll
         for (int k = UR - 1; k >= 0; --k) {
           const int r = r0 + k;
-          const float2 u = du[r * 64 + lane];
+          const float2 u = make_float2(sd[r * 64 + lane], sx[r * 64 + lane]);
           const float e = se[r * 64 + lane];
           float p = 0.f, q = 0.f, red[2 * NS];
 #pragma unroll
@@ -522,7 +534,8 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
             q = fmaf(t, A1[i], q);
             dAt[i] = fmaf(t, u.x, dAt[i]);
           }
-          pq[(w * TQ + r) * 64 + lane] = make_float2(p, q);
+          pp[(w * TQ + r) * 64 + lane] = p;
+          pq[(w * TQ + r) * 64 + lane] = q;
           const float s = lanes_sum<2 * NS>(red, lane);
           sbc[col + r * row] = s;
         }
@@ -537,30 +550,34 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
         const int r = me.r[i];
         if (r >= TQ) continue;
         const bool in = s0 + r < len;
+        const int at = r * 64 + me.cl;
         float p[V], q[V], v[V];
 #pragma unroll
         for (int k = 0; k < V; ++k) p[k] = q[k] = v[k] = 0.f;
+        auto add = [&](int u) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (u < a.W)
+          for (int k = 0; k < V; ++k) {
+            p[k] += pp[u * TQ * 64 + at + k];
+            q[k] += pq[u * TQ * 64 + at + k];
+            v[k] += yp[u * TQ * 64 + at + k];
+          }
+        };
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-              const float2 t = pq[(u * TQ + r) * 64 + me.cl + k];
-              p[k] += t.x;
-              q[k] += t.y;
-              if (gate) v[k] += yp[(u * TQ + r) * 64 + me.cl + k];
-            }
+        for (int u = 0; u < 4; ++u) add(u);  // W >= 4
+        for (int u = 4; u < a.W; ++u) add(u);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float x = in ? cx[i][k] : 0.f, e = se[r * 64 + me.cl + k], dt = du[r * 64 + me.cl + k].x;
-          float dd = fmaf(x, p[k], q[k]);
-          if (a.softplus) dd *= sigmoidf(cd[i][k] + bias[k]);
-          ox[i][k] = in ? fmaf(dt, p[k], skip[k] * e) : 0.f;
-          od[i][k] = in ? dd : 0.f;
-          oz[i][k] = in && gate ? cy[i][k] * fmaf(skip[k], x, v[k]) * dsiluf(cz[i][k]) : 0.f;
+          const float x = in ? cx[i][k] : 0.f, e = se[at + k];
+          const float sg = sigmoidf(cd[i][k] + bias[k]), dd = fmaf(x, p[k], q[k]);
+          ox[i][k] = in ? fmaf(sd[at + k], p[k], skip[k] * e) : 0.f;
+          od[i][k] = in ? (a.softplus ? dd * sg : dd) : 0.f;
+          v[k] = fmaf(skip[k], x, v[k]);
           gskip[k] = fmaf(e, x, gskip[k]);
           gbias[k] += od[i][k];
         }
+        if (gate)
+#pragma unroll
+          for (int k = 0; k < V; ++k) oz[i][k] = in ? cy[i][k] * v[k] * dsiluf(cz[i][k]) : 0.f;
       }
       // (a thread stages the elements that it has just read)
       if (more) stage(s0 - TQ);
