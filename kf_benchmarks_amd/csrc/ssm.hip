@@ -152,6 +152,13 @@ __device__ __forceinline__ void params(const float* p, int c, bool on, float (&v
   for (int k = 0; k < V; ++k) v[k] = on && p ? p[c + k] : 0.f;
 }
 
+// V neighbouring floats of LDS at once (V = 4: 16-byte aligned)
+template <int V> struct alignas(4 * V) Quad {
+  float v[V];
+};
+template <int V> __device__ __forceinline__ Quad<V> get(const float* p) { return *(const Quad<V>*)p; }
+template <int V> __device__ __forceinline__ void put(float* p, const Quad<V>& q) { *(Quad<V>*)p = q; }
+
 __device__ __forceinline__ float step_size(float raw, bool softplus) {
   const float v = softplusf(raw);  // (a select, not a branch: the flag is uniform)
   return softplus ? v : raw;
@@ -187,7 +194,7 @@ __device__ __forceinline__ void join(const Args& a, int b, int dc, long bnd, lon
 // ENDS: only the state after each chunk, from zero, and the chunk's sum of dt.
 template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
-  extern __shared__ float lds[];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;  // steps of a group
   float *sd = lds, *sx = lds + TQ * 64;  // [TQ][64] dt, dt x
   float* yp = lds + TQ * 64 * 2;         // [W][TQ][64]
@@ -225,12 +232,15 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
       if (me.r[i] < TQ) {
         const bool in = me.on && s0 + me.r[i] < len;
         const int at = me.r[i] * 64 + me.cl;
+        Quad<V> qd, qx;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const float dt = step_size(nd[i][k] + bias[k], a.softplus);
-          sd[at + k] = in ? dt : 0.f;
-          sx[at + k] = in ? dt * nx[i][k] : 0.f;
+          qd.v[k] = in ? dt : 0.f;
+          qx.v[k] = in ? dt * nx[i][k] : 0.f;
         }
+        put(sd + at, qd);
+        put(sx + at, qx);
       }
   };
   float sum_dt = 0.f;
@@ -283,12 +293,16 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
           for (int k = 0; k < V; ++k) v[k] = skip[k] * cx[i][k];
           const float* part = yp + r * 64 + me.cl;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)  // W >= 4
+          for (int q = 0; q < 4; ++q) {  // W >= 4
+            const Quad<V> t = get<V>(part + q * TQ * 64);
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[k] += part[q * TQ * 64 + k];
-          for (int q = 4; q < a.W; ++q)
+            for (int k = 0; k < V; ++k) v[k] += t.v[k];
+          }
+          for (int q = 4; q < a.W; ++q) {
+            const Quad<V> t = get<V>(part + q * TQ * 64);
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[k] += part[q * TQ * 64 + k];
+            for (int k = 0; k < V; ++k) v[k] += t.v[k];
+          }
           if (gate)
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] *= siluf(cz[i][k]);
@@ -379,7 +393,7 @@ template <int M> __device__ __forceinline__ int lane_value(int l) {
 // ENDS: only the gradient before each chunk, from zero behind it, and sum dt.
 template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
-  extern __shared__ float lds[];
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const int WN = a.W * NS;
   constexpr int UR = 8 / NS < 4 ? 8 / NS : 4;
   float *sd = lds, *sx = lds + TQ * 64, *se = lds + TQ * 64 * 2;  // [TQ][64] dt, dt x, e
@@ -441,13 +455,17 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
         if (gate)
 #pragma unroll
           for (int k = 0; k < V; ++k) e[k] *= siluf(nz[i][k]);
+        Quad<V> qd, qx, qe;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           const float dt = step_size(nd[i][k] + bias[k], a.softplus);
-          sd[at + k] = in ? dt : 0.f;
-          if (!ENDS) sx[at + k] = in ? dt * nx[i][k] : 0.f;
-          se[at + k] = in ? e[k] : 0.f;
+          qd.v[k] = in ? dt : 0.f;
+          qx.v[k] = in && !ENDS ? dt * nx[i][k] : 0.f;
+          qe.v[k] = in ? e[k] : 0.f;
         }
+        put(sd + at, qd);
+        if (!ENDS) put(sx + at, qx);
+        put(se + at, qe);
       }
       cx[i] = nx[i];
       cd[i] = nd[i];
@@ -555,21 +573,24 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
 #pragma unroll
         for (int k = 0; k < V; ++k) p[k] = q[k] = v[k] = 0.f;
         auto add = [&](int u) {
+          const Quad<V> tp = get<V>(pp + u * TQ * 64 + at), tq = get<V>(pq + u * TQ * 64 + at),
+                        tv = get<V>(yp + u * TQ * 64 + at);
 #pragma unroll
           for (int k = 0; k < V; ++k) {
-            p[k] += pp[u * TQ * 64 + at + k];
-            q[k] += pq[u * TQ * 64 + at + k];
-            v[k] += yp[u * TQ * 64 + at + k];
+            p[k] += tp.v[k];
+            q[k] += tq.v[k];
+            v[k] += tv.v[k];
           }
         };
 #pragma unroll
         for (int u = 0; u < 4; ++u) add(u);  // W >= 4
         for (int u = 4; u < a.W; ++u) add(u);
+        const Quad<V> me_d = get<V>(sd + at), me_e = get<V>(se + at);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float x = in ? cx[i][k] : 0.f, e = se[at + k];
+          const float x = in ? cx[i][k] : 0.f, e = me_e.v[k];
           const float sg = sigmoidf(cd[i][k] + bias[k]), dd = fmaf(x, p[k], q[k]);
-          ox[i][k] = in ? fmaf(sd[at + k], p[k], skip[k] * e) : 0.f;
+          ox[i][k] = in ? fmaf(me_d.v[k], p[k], skip[k] * e) : 0.f;
           od[i][k] = in ? (a.softplus ? dd * sg : dd) : 0.f;
           v[k] = fmaf(skip[k], x, v[k]);
           gskip[k] = fmaf(e, x, gskip[k]);

@@ -15,6 +15,7 @@ Layouts:
 from __future__ import annotations
 
 import contextlib
+import functools
 import math
 import os
 from typing import Optional, Sequence, Tuple
@@ -607,12 +608,26 @@ def check_params(x, shape, **params):
             raise ValueError("%s is on %s, the input on %s" % (name, p.device, x.device))
 
 
+def fits_param(t, shape, dev):
+    """check_params' conditions, as one answer"""
+    return t is None or (t.shape == shape and t.dtype is torch.float32 and t.device == dev
+                         and t.is_contiguous())
+
+
+@functools.lru_cache(maxsize=4096)
+def size_query(name, *args):
+    """A size that a native entry point derives from its (integer) arguments."""
+    return N.query(name, *args)
+
+
 def on_device(x):
     """Context in which ``x``'s device is the current one (kernels launch on
     the current device, whatever stream they are given)."""
-    if x.device.index is None or x.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(x.device)
+    i = x.get_device()
+    return _SAME_DEVICE if i == torch._C._cuda_getDevice() else torch.cuda.device(i)
+
+
+_SAME_DEVICE = contextlib.nullcontext()
 
 
 N.register_optional("kfb_gn_fwd_ws", [N.I, N.L, N.L, N.I, N.I], N.L)
@@ -626,12 +641,13 @@ N.register_optional("kfb_gn_bwd", [N.I, N.P, N.P, N.P, N.L, N.L, N.I, N.I, N.P, 
 def _gn_forward(x, gamma, beta, groups, eps, act):
     C, n = x.shape[-1], x.shape[0]
     hw = x.numel() // (n * C)
+    dt = N.dt(x)
     y = torch.empty_like(x)
-    nws = N.query("kfb_gn_fwd_ws", N.dt(x), n, hw, C, groups)
-    st = torch.empty((2 * n * groups + nws,), dtype=torch.float32, device=x.device)
+    st = x.new_empty((2 * n * groups + size_query("kfb_gn_fwd_ws", dt, n, hw, C, groups),),
+                     dtype=torch.float32)
     base = st.data_ptr()
-    N.call("kfb_gn_fwd", N.dt(x), x.data_ptr(), y.data_ptr(), n, hw, C, groups, N.ptr(gamma),
-           N.ptr(beta), float(eps), act, base, base + 4 * n * groups, base + 8 * n * groups,
+    N.call("kfb_gn_fwd", dt, x.data_ptr(), y.data_ptr(), n, hw, C, groups, N.ptr(gamma),
+           N.ptr(beta), eps, act, base, base + 4 * n * groups, base + 8 * n * groups,
            N.stream(x.device))
     return y, st
 
@@ -658,8 +674,8 @@ class _GroupNorm(torch.autograd.Function):
         grads = [s if s is not None or p is None else torch.empty((C,), dtype=torch.float32,
                                                                   device=dev)
                  for s, p in zip(sinks, ctx.params)]
-        ws = torch.empty((N.query("kfb_gn_bwd_ws", N.dt(x), n, hw, C, groups),),
-                         dtype=torch.float32, device=dev)
+        ws = x.new_empty((size_query("kfb_gn_bwd_ws", N.dt(x), n, hw, C, groups),),
+                         dtype=torch.float32)
         base = st.data_ptr()
         N.call("kfb_gn_bwd", N.dt(x), dy.data_ptr(), x.data_ptr(), dx.data_ptr(), n, hw, C, groups,
                N.ptr(gamma), N.ptr(beta), act, base, base + 4 * n * groups, N.ptr(grads[0]),
@@ -689,7 +705,9 @@ def group_norm(x, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], g
     C = x.shape[-1]
     if groups < 1 or C % groups:
         raise ValueError("group_norm: %d channels do not split into %d groups" % (C, groups))
-    check_params(x, (C,), gamma=gamma, beta=beta)
+    dev = x.device
+    if not (fits_param(gamma, (C,), dev) and fits_param(beta, (C,), dev)):
+        check_params(x, (C,), gamma=gamma, beta=beta)
     if not _on_gpu(x):
         y = x.float().reshape(x.shape[0], -1, groups, C // groups)
         v, m = torch.var_mean(y, dim=(1, 3), unbiased=False, keepdim=True)
@@ -697,13 +715,14 @@ def group_norm(x, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], g
         y = y * gamma if gamma is not None else y
         y = y + beta if beta is not None else y
         return apply_act(y, activation).to(x.dtype)
-    N.dt(x)
     x = x.contiguous()
+    grad = torch.is_grad_enabled() and (x.requires_grad or
+                                        (gamma is not None and gamma.requires_grad) or
+                                        (beta is not None and beta.requires_grad))
     with on_device(x):
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (x, gamma, beta)):
-            return _GroupNorm.apply(x, gamma, beta, int(groups), eps, act)
-        return _gn_forward(x, gamma, beta, int(groups), eps, act)[0]
+        if grad:
+            return _GroupNorm.apply(x, gamma, beta, int(groups), float(eps), act)
+        return _gn_forward(x, gamma, beta, int(groups), float(eps), act)[0]
 
 
 # -------------------------------------------------------------- bias + relu

@@ -87,7 +87,21 @@ def _check_lengths(x, lengths):
 
 
 def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _fits(t, shape, dtype, dev):
+    return t is None or (t.shape == shape and t.dtype is dtype and t.device == dev)
+
+
+def _rows2(t):
+    """_rows of a [B, K] tensor."""
+    s0, s1 = t.stride()
+    return (t, s0) if s1 == 1 or t.shape[1] == 1 else (t.contiguous(), t.shape[1])
 
 
 def _grad_buffers(params):
@@ -176,7 +190,7 @@ class _CausalConv(torch.autograd.Function):
         dx = torch.empty((T, B, D), dtype=x.dtype, device=dev)
         dinit = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[3] else None
         grads, acc = _grad_buffers(ctx.params)
-        ws = torch.empty((N.query("kfb_cconv_bwd_ws", T, B, D, K),), dtype=torch.float32, device=dev)
+        ws = torch.empty((F_ops.size_query("kfb_cconv_bwd_ws", T, B, D, K),), dtype=torch.float32, device=dev)
         N.call("kfb_cconv_bwd", N.dt(x),
                int(_vec(D, 4, (x, ldx), (dy, ldy), (initial, D), (dlast, D))), dy.data_ptr(), ldy,
                x.data_ptr(), ldx, N.ptr(initial), w.data_ptr(), N.ptr(b), N.ptr(lengths),
@@ -235,10 +249,16 @@ def causal_conv_step(x, state, w, b=None, activation=None):
     if x.dim() != 2 or x.numel() == 0:
         raise ValueError("causal_conv_step: a non-empty [B, D] tensor expected, got %s" %
                          (tuple(x.shape),))
-    _check_conv(x, w, b)
     B, D = x.shape
-    K = w.shape[0]
-    _same(x, (K - 1, B, D), state=state)
+    K, dt, dev = w.shape[0], x.dtype, x.device
+    # (one token: the checks are a good part of the call, so the messages are left
+    # to the slow ones)
+    if not (1 <= K <= MAX_TAPS and F_ops.fits_param(w, (K, D), dev) and F_ops.fits_param(b, (D,), dev)
+            and _fits(state, (K - 1, B, D), dt, dev) and state is not None):
+        _check_conv(x, w, b)
+        if state is None:
+            raise ValueError("causal_conv_step: a state expected")
+        _same(x, (K - 1, B, D), state=state)
     if not state.is_contiguous():
         raise ValueError("causal_conv_step: a contiguous state expected")
     if _needs_grad(x, state, w, b):
@@ -248,13 +268,12 @@ def causal_conv_step(x, state, w, b=None, activation=None):
         y, last = causal_conv_reference(x[None], w, b, activation, None, state)
         state.copy_(last)
         return y[0]
+    x, ld = _rows2(x)
+    y = x.new_empty((B, D))
+    px, ps, ve = x.data_ptr(), state.data_ptr(), 4 if dt is torch.float32 else 8
     with F_ops.on_device(x):
-        x, ld = _rows(x)
-        y = torch.empty((B, D), dtype=x.dtype, device=x.device)
-        ve = 16 // x.element_size()
-        N.call("kfb_cconv_step", N.dt(x), int(_vec(D, ve, (x, ld), (state, D))), x.data_ptr(), ld,
-               state.data_ptr(), w.data_ptr(), N.ptr(b), y.data_ptr(), B, D, K, act,
-               N.stream(x.device))
+        N.call("kfb_cconv_step", N.dt(x), int(D % ve == 0 and ld % ve == 0 and (px | ps) % 16 == 0),
+               px, ld, ps, w.data_ptr(), N.ptr(b), y.data_ptr(), B, D, K, act, N.stream(dev))
     return y
 
 
@@ -297,8 +316,8 @@ def _scan_forward(x, delta, A, B, C, D, z, bias, lengths, h0, softplus, reverse,
     y = torch.empty((T, Bn, Dn), dtype=x.dtype, device=dev)
     f32 = dict(dtype=torch.float32, device=dev)
     hT = torch.empty((Bn, Ns, Dn), **f32) if state else None
-    bc = torch.empty((N.query("kfb_ssm_floats", 0, T, Bn, Dn, Ns),), **f32)
-    hs = torch.empty((N.query("kfb_ssm_floats", 1, T, Bn, Dn, Ns),), **f32) if train else None
+    bc = torch.empty((F_ops.size_query("kfb_ssm_floats", 0, T, Bn, Dn, Ns),), **f32)
+    hs = torch.empty((F_ops.size_query("kfb_ssm_floats", 1, T, Bn, Dn, Ns),), **f32) if train else None
     V = 4 if _vec(Dn, 4, (x, ldx), (delta, ldd), (z, ldz)) else 1
     N.call("kfb_ssm_scan_fwd", N.dt(x), V, x.data_ptr(), ldx, delta.data_ptr(), ldd, N.ptr(z), ldz,
            B.data_ptr(), ldb, C.data_ptr(), ldc, A.data_ptr(), N.ptr(D), N.ptr(bias),
@@ -336,7 +355,7 @@ class _SelectiveScan(torch.autograd.Function):
         dz = torch.empty((T, Bn, Dn), dtype=dt, device=dev) if z is not None else None
         dB, dC = (torch.empty((T, Bn, Ns), dtype=dt, device=dev) for _ in range(2))
         grads, acc = _grad_buffers(ctx.params)
-        ws = torch.empty((N.query("kfb_ssm_floats", 2, T, Bn, Dn, Ns),), **f32)
+        ws = torch.empty((F_ops.size_query("kfb_ssm_floats", 2, T, Bn, Dn, Ns),), **f32)
         V = 4 if _vec(Dn, 4, (x, ldx), (delta, ldd), (z, ldz), (dy, ldy)) else 1
         N.call("kfb_ssm_scan_bwd", N.dt(x), V, dy.data_ptr(), ldy, x.data_ptr(), ldx,
                delta.data_ptr(), ldd, N.ptr(z), ldz, A.data_ptr(), N.ptr(D), N.ptr(bias),
@@ -381,9 +400,14 @@ def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     if x.dim() != 3 or x.numel() == 0:
         raise ValueError("selective_scan: a non-empty [T, B, D] tensor expected, got %s" %
                          (tuple(x.shape),))
-    _check_scan(x, delta, A, B, C, D, z, delta_bias)
+    T, Bn, Dn = shape = x.shape
+    dt, dev, Ns = x.dtype, x.device, A.shape[0]
+    if not (1 <= Ns <= MAX_STATES and _fits(delta, shape, dt, dev) and _fits(z, shape, dt, dev)
+            and _fits(B, (T, Bn, Ns), dt, dev) and _fits(C, (T, Bn, Ns), dt, dev)
+            and F_ops.fits_param(A, (Ns, Dn), dev) and F_ops.fits_param(D, (Dn,), dev)
+            and F_ops.fits_param(delta_bias, (Dn,), dev)):
+        _check_scan(x, delta, A, B, C, D, z, delta_bias)
     _check_lengths(x, lengths)
-    T, Bn, Dn = x.shape
     _check_state(x, Bn, A.shape[0], Dn, initial_state=initial_state)
     if not x.is_cuda:
         y, h = selective_scan_reference(x, delta, A, B, C, D, z, delta_bias, softplus, lengths,
@@ -407,10 +431,20 @@ def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     if x.dim() != 2 or x.numel() == 0:
         raise ValueError("selective_scan_step: a non-empty [B, D] tensor expected, got %s" %
                          (tuple(x.shape),))
-    _check_scan(x, delta, A, B, C, D, z, delta_bias)
-    Bn, Dn = x.shape
+    shape, dt, dev = x.shape, x.dtype, x.device
+    Bn, Dn = shape
     Ns = A.shape[0]
-    _check_state(x, Bn, Ns, Dn, state=state)
+    if not (1 <= Ns <= MAX_STATES and Bn <= 65535 and _fits(delta, shape, dt, dev)
+            and _fits(z, shape, dt, dev) and _fits(B, (Bn, Ns), dt, dev)
+            and _fits(C, (Bn, Ns), dt, dev) and F_ops.fits_param(A, (Ns, Dn), dev)
+            and F_ops.fits_param(D, (Dn,), dev) and F_ops.fits_param(delta_bias, (Dn,), dev)
+            and state is not None and F_ops.fits_param(state, (Bn, Ns, Dn), dev)):
+        _check_scan(x, delta, A, B, C, D, z, delta_bias)
+        if state is None:
+            raise ValueError("selective_scan_step: a state expected")
+        _check_state(x, Bn, Ns, Dn, state=state)
+        if x.is_cuda:
+            raise ValueError("selective_scan_step: at most 65535 sequences, got %d" % Bn)
     if _needs_grad(x, delta, A, B, C, state, D, z, delta_bias):
         raise ValueError("selective_scan_step updates its state in place and has no gradient: "
                          "call it under torch.no_grad()")
@@ -420,13 +454,11 @@ def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=Non
                                         None, state)
         state.copy_(h)
         return y[0]
-    if Bn > 65535:
-        raise ValueError("selective_scan_step: at most 65535 sequences, got %d" % Bn)
+    (x, ldx), (delta, ldd), (B, ldb), (C, ldc) = _rows2(x), _rows2(delta), _rows2(B), _rows2(C)
+    z, ldz = _rows2(z) if z is not None else (None, 0)
+    y = x.new_empty((Bn, Dn))
     with F_ops.on_device(x):
-        (x, ldx), (delta, ldd), (B, ldb), (C, ldc) = _rows(x), _rows(delta), _rows(B), _rows(C)
-        z, ldz = _rows(z) if z is not None else (None, 0)
-        y = torch.empty((Bn, Dn), dtype=x.dtype, device=x.device)
         N.call("kfb_ssm_step", N.dt(x), x.data_ptr(), ldx, delta.data_ptr(), ldd, N.ptr(z), ldz,
                B.data_ptr(), ldb, C.data_ptr(), ldc, A.data_ptr(), N.ptr(D), N.ptr(delta_bias),
-               state.data_ptr(), y.data_ptr(), Bn, Dn, Ns, int(softplus), N.stream(x.device))
+               state.data_ptr(), y.data_ptr(), Bn, Dn, Ns, int(softplus), N.stream(dev))
     return y
