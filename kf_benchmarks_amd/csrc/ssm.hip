@@ -1,6 +1,7 @@
 // Selective state space scan over time-major sequences [T][B][D] with N states
 // per channel, h [B][N][D] fp32:
 //   dt = softplus(delta + bias)            (or delta + bias)
+//   A = -exp(A)                            (with log_a, or as given)
 //   h_t = exp(dt A) h_{t-1} + dt x B_t
 //   y   = (sum_n C_t h_t + skip x) silu(z)
 // A [N][D], skip, bias [D] fp32; B, C [T][B][N] of x's type.  Position s of a
@@ -47,7 +48,7 @@ struct Args {
   // zero [nchunk][B][N][D], sum of dt [nchunk][B][D]
   float *ends, *sums;
   int nchunk, tpc;
-  int T, B, D, N, W, Tp, softplus, reverse;
+  int T, B, D, N, W, Tp, softplus, reverse, log_a;
 };
 
 // B and C as constant memory: uniform addresses become scalar loads
@@ -72,6 +73,10 @@ template <int NS, int UR> struct Group {
 };
 
 constexpr int BC_PAD = 64;  // floats behind bc: a group is fetched ahead
+
+__device__ __forceinline__ float rate(const Args& a, long i) {
+  return a.log_a ? -expf(a.A[i]) : a.A[i];
+}
 
 __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.T) : a.T;
@@ -207,7 +212,7 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   float A2[NS], h[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    A2[i] = i < ns ? a.A[(long)(w * NS + i) * a.D + dc] * LOG2E : 0.f;
+    A2[i] = i < ns ? rate(a, (long)(w * NS + i) * a.D + dc) * LOG2E : 0.f;
     h[i] = i < ns && a.h0 && !ENDS ? a.h0[bnd + (long)i * a.D] : 0.f;
   }
   if constexpr (!ENDS) join<NS>(a, b, dc, bnd, bn, ns, A2, 0, 1, chunk, h);
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   float A1[NS], carry[NS], dA[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
-    A1[i] = i < ns && ok ? a.A[(long)(w * NS + i) * a.D + dc] : 0.f;
+    A1[i] = i < ns && ok ? rate(a, (long)(w * NS + i) * a.D + dc) : 0.f;
     carry[i] = i < ns && ok && a.dhT && !ENDS ? a.dhT[bnd + (long)i * a.D] : 0.f;
     dA[i] = 0.f;
   }
@@ -677,8 +682,8 @@ bc_grad_k(const float* __restrict__ p, int nblk, long rows, int N, T* __restrict
 // dA [N][D], dskip, dbias [D]: the sum over the slabs of pch [S][N + 2][D], 32
 // columns x 8 rows a workgroup
 __global__ void __launch_bounds__(256)
-param_grad_k(const float* __restrict__ p, int S, int N, int D, float* dA, float* dskip,
-             float* dbias, int acc_a, int acc_s, int acc_b) {
+param_grad_k(const float* __restrict__ p, int S, int N, int D, const float* log_a, float* dA,
+             float* dskip, float* dbias, int acc_a, int acc_s, int acc_b) {
   __shared__ float red[8][33];
   const long total = (long)(N + 2) * D;
   const int cl = threadIdx.x % 32, r0 = threadIdx.x / 32;
@@ -699,6 +704,7 @@ param_grad_k(const float* __restrict__ p, int S, int N, int D, float* dA, float*
   float* out = n < N ? dA : n == N ? dskip : dbias;
   const int acc = n < N ? acc_a : n == N ? acc_s : acc_b;
   if (!out) return;
+  if (n < N && log_a) sum *= -expf(log_a[i]);
   out += n < N ? i : i % D;
   *out = acc ? *out + sum : sum;
 }
@@ -721,7 +727,7 @@ __global__ void __launch_bounds__(256) step_k(Args a, float* __restrict__ state)
     for (int n = w; n < a.N; n += 4) {
       const float B = to_f32(((const T*)a.bm)[b * a.ldb + n]);
       const float C = to_f32(((const T*)a.cm)[b * a.ldc + n]);
-      const float e = __builtin_amdgcn_exp2f(dt * (a.A[(long)n * a.D + d] * LOG2E));
+      const float e = __builtin_amdgcn_exp2f(dt * (rate(a, (long)n * a.D + d) * LOG2E));
       const float u = fmaf(e, h[(long)n * a.D], dt * x * B);
       h[(long)n * a.D] = u;
       v = fmaf(C, u, v);
@@ -815,13 +821,13 @@ KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V_, const void* x, long ldx, 
                                     const void* cm, long ldc, const float* A, const float* skip,
                                     const float* bias, const int* len, const float* h0, float* hT,
                                     float* hs, float* bc, void* y, int T, int B, int D, int N,
-                                    int softplus, int reverse, hipStream_t stream) {
+                                    int softplus, int reverse, int log_a, hipStream_t stream) {
   ssm::Args a{};
   a.x = x; a.delta = delta; a.z = z; a.bm = bm; a.cm = cm;
   a.ldx = ldx; a.ldd = ldd; a.ldz = ldz; a.ldb = ldb; a.ldc = ldc;
   a.A = A; a.skip = skip; a.bias = bias; a.len = len; a.h0 = h0; a.hT = hT; a.hs = hs; a.bc = bc;
   a.y = y;
-  a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse;
+  a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse; a.log_a = log_a;
   if (ssm::bad(a) || (V_ != 1 && V_ != 4)) return hipErrorInvalidValue;
   const ssm::Plan p = ssm::plan(T, B, D, N);
   a.W = p.W; a.Tp = p.Tp;
@@ -850,13 +856,13 @@ KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V_, const void* dy, long ldy,
                                     float* dh0, void* dx, void* ddelta, void* dz, void* db,
                                     void* dc, float* dA, float* dskip, float* dbias, int acc_a,
                                     int acc_skip, int acc_bias, float* ws, int T, int B, int D,
-                                    int N, int softplus, int reverse, hipStream_t stream) {
+                                    int N, int softplus, int reverse, int log_a, hipStream_t stream) {
   ssm::Args a{};
   a.x = x; a.delta = delta; a.z = z; a.dy = dy;
   a.ldx = ldx; a.ldd = ldd; a.ldz = ldz; a.ldy = ldy;
   a.A = A; a.skip = skip; a.bias = bias; a.len = len; a.hs = const_cast<float*>(hs); a.bc = bc;
   a.dhT = dhT; a.dh0 = dh0; a.dx = dx; a.ddelta = ddelta; a.dz = dz;
-  a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse;
+  a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse; a.log_a = log_a;
   if (ssm::bad(a) || (V_ != 1 && V_ != 4) || !ws || !hs) return hipErrorInvalidValue;
   const ssm::Plan p = ssm::plan(T, B, D, N);
   a.W = p.W; a.Tp = p.Tp;
@@ -883,7 +889,7 @@ KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V_, const void* dy, long ldy,
                        dim3(256), 0, stream, a.pbc, nblk, rows, N, (E*)db, (E*)dc);
   });
   hipLaunchKernelGGL(ssm::param_grad_k, dim3(ceil_div((long)(N + 2) * D, 32)), dim3(256), 0, stream,
-                     a.pch, B * a.nchunk, N, D, dA, dskip, dbias, acc_a, acc_skip, acc_bias);
+                     a.pch, B * a.nchunk, N, D, log_a ? A : nullptr, dA, dskip, dbias, acc_a, acc_skip, acc_bias);
   return hipGetLastError();
 }
 
@@ -891,12 +897,12 @@ KFB_API hipError_t kfb_ssm_step(int dtype, const void* x, long ldx, const void* 
                                 const void* z, long ldz, const void* bm, long ldb, const void* cm,
                                 long ldc, const float* A, const float* skip, const float* bias,
                                 float* state, void* y, int B, int D, int N, int softplus,
-                                hipStream_t stream) {
+                                int log_a, hipStream_t stream) {
   ssm::Args a{};
   a.x = x; a.delta = delta; a.z = z; a.bm = bm; a.cm = cm;
   a.ldx = ldx; a.ldd = ldd; a.ldz = ldz; a.ldb = ldb; a.ldc = ldc;
   a.A = A; a.skip = skip; a.bias = bias; a.y = y;
-  a.T = 1; a.B = B; a.D = D; a.N = N; a.softplus = softplus;
+  a.T = 1; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.log_a = log_a;
   if (ssm::bad(a)) return hipErrorInvalidValue;
   KFB_DISPATCH_DTYPE(dtype, E, {
     hipLaunchKernelGGL((ssm::step_k<E>), dim3(ceil_div(D, 64), B), dim3(256), 0, stream, a, state);

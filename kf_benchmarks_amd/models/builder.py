@@ -28,7 +28,8 @@ from .. import ops
 from ..ops import _native as N
 from ..ops import conv as conv_ops
 from ..ops import nn as F
-from .layers import AffineLayer, BatchNormLayer, ConvLayer, DepthwiseConvLayer
+from .layers import (AffineLayer, BatchNormLayer, ConvLayer, DepthwiseConvLayer,
+                     GroupNormLayer)
 
 
 # Independent branches (ResNet projection shortcuts) on a side stream: off
@@ -490,6 +491,23 @@ class ConvNetBuilder:
             y = F.batch_norm(x, layer.gamma, layer.beta, layer.moving_mean,
                              layer.moving_variance, layer.decay, layer.eps, training, relu,
                              residual, stats=stats if training else None)
+        self.top_layer, self.top_size = y, C
+        return y
+
+    def group_norm(self, groups=32, input_layer=None, scale=True, epsilon=1e-5,
+                   activation=None):
+        """Group norm of NHWC images with a fused activation (ops.nn.group_norm):
+        the same function in training and in evaluation."""
+        x = self.top_layer if input_layer is None else input_layer
+        self._use(x)
+        C = x.shape[-1]
+        name = "groupnorm%d" % self.counts["groupnorm"]
+        self.counts["groupnorm"] += 1
+        scope = self._scoped(name)
+        layer = self._layer(scope, lambda: GroupNormLayer(scope, C, groups, scale, epsilon,
+                                                          self.net.param_device))
+        y = F.group_norm(x, self._p(layer.gamma), self._p(layer.beta), layer.groups, layer.eps,
+                         activation)
         self.top_layer, self.top_size = y, C
         return y
 

@@ -22,6 +22,7 @@ from torch import nn
 from .. import cnn_util
 from ..ops import nn as F_ops
 from ..ops import rnn as rnn_ops
+from ..ops import ssm as ssm_ops
 from . import model as model_lib
 
 SPEECH_LABELS = " abcdefghijklmnopqrstuvwxyz'-"
@@ -133,6 +134,49 @@ class _RNNLayer(nn.Module):
                                  wx_lp=getattr(self.wx, "_kfb_lp", None))
 
 
+class _SSMLayer(nn.Module):
+    """One (bi)directional selective state space layer (ops.ssm.ssm_layer), a
+    direction's parameters of its own, outputs side by side as the recurrent
+    layers'.  16 states a channel, a convolution of 4 frames, step sizes through
+    a rank of hidden / 16; decays -1..-16, step sizes log-uniform in [0.001, 0.1]
+    at the start.  Its group norm (per frame) stands for the batch norm."""
+
+    STATES, TAPS = 16, 4
+    MATRICES = ("w_in", "w_rank", "w_delta", "w_bc")
+
+    def __init__(self, din, hidden, dirs, gen, device):
+        super().__init__()
+        self.dirs = dirs
+        self.groups = next(g for g in (8, 4, 2, 1) if hidden % g == 0)
+        rank = -(-hidden // 16)
+        N, K = self.STATES, self.TAPS
+
+        def uniform(a, b):
+            lim = (6.0 / (a + b)) ** 0.5
+            return (torch.rand((a, b), generator=gen) * 2 - 1) * lim
+
+        for d in range(dirs):
+            step = torch.exp(torch.rand(hidden, generator=gen) * np.log(100.0) + np.log(0.001))
+            for name, v in (("w_in", uniform(din, 2 * hidden)), ("w_rank", uniform(hidden, rank)),
+                            ("w_delta", uniform(rank, hidden)), ("w_bc", uniform(hidden, 2 * N)),
+                            ("conv_w", torch.randn((K, hidden), generator=gen) / K ** 0.5),
+                            ("conv_b", torch.zeros(hidden)), ("D", torch.ones(hidden)),
+                            ("A_log", torch.log(torch.arange(1.0, N + 1))[:, None].repeat(1, hidden)),
+                            ("delta_bias", step + torch.log(-torch.expm1(-step))),
+                            ("norm_w", torch.ones(hidden))):
+                setattr(self, "%s_%d" % (name, d), nn.Parameter(v.to(device)))
+
+    def forward(self, x):  # [T, B, din] -> [T, B, dirs*H]
+        out = []
+        for d, xd in enumerate(F_ops.fanout(x, self.dirs)):
+            p = {name: getattr(self, "%s_%d" % (name, d)) for name in (
+                "w_in", "conv_w", "conv_b", "w_rank", "w_delta", "w_bc", "delta_bias", "A_log",
+                "D", "norm_w")}
+            low = {name: getattr(p[name], "_kfb_lp", None) for name in self.MATRICES}
+            out.append(ssm_ops.ssm_layer(xd, **p, groups=self.groups, reverse=d == 1, low=low))
+        return F_ops.concat_channels(out)
+
+
 class DeepSpeech2(nn.Module):
     def __init__(self, nclass, num_rnn_layers, rnn_type, bidirectional, hidden, use_bias,
                  feature_bins, gen, device):
@@ -141,12 +185,17 @@ class DeepSpeech2(nn.Module):
         self.conv2 = _ConvBN(32, 32, (21, 11), (2, 1), (10, 5), gen, device)
         f = (feature_bins + 10 - 11) // 2 + 1
         f = (f + 10 - 11) // 1 + 1
-        kind = rnn_ops._KIND[rnn_type]
+        kind = rnn_ops._KIND.get(rnn_type)
         dirs = 2 if bidirectional else 1
         self.rnns = nn.ModuleList()
         self.bns = nn.ModuleList()
         din = f * 32
         for i in range(num_rnn_layers):
+            if rnn_type == "ssm":
+                self.bns.append(nn.Identity())
+                self.rnns.append(_SSMLayer(din, hidden, dirs, gen, device))
+                din = hidden * dirs
+                continue
             self.bns.append(_BN(din, device) if i > 0 else nn.Identity())
             self.rnns.append(_RNNLayer(din, hidden, kind, dirs, gen, device))
             din = hidden * dirs
@@ -175,7 +224,7 @@ class DeepSpeech2(nn.Module):
 
 
 class DeepSpeech2Model(model_lib.ModuleModel):
-    SUPPORTED_RNNS = ("lstm", "rnn", "gru")
+    SUPPORTED_RNNS = ("lstm", "rnn", "gru", "ssm")
     BATCH_NORM_EPSILON = 1e-5
     BATCH_NORM_DECAY = 0.997
     CONV_FILTERS = 32

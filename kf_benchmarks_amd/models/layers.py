@@ -154,6 +154,26 @@ class BatchNormLayer(Layer):
             getattr(self, name).copy_(t)
 
 
+class GroupNormLayer(Layer):
+    def __init__(self, scope, channels, groups, scale, eps, device):
+        super().__init__()
+        self.tf_scope = scope
+        self.groups, self.eps = int(groups), float(eps)
+        self.gamma = nn.Parameter(torch.ones(channels, device=device)) if scale else None
+        self.beta = nn.Parameter(torch.zeros(channels, device=device))
+
+    def tf_variables(self):
+        out = {"beta": self.beta.detach()}
+        if self.gamma is not None:
+            out["gamma"] = self.gamma.detach()
+        return out
+
+    def load_tf_variable(self, name, value):
+        t = torch.as_tensor(value, dtype=torch.float32)
+        with torch.no_grad():
+            getattr(self, name).copy_(t)
+
+
 class AffineLayer(Layer):
     """weights [Cin, Cout] (TF layout, used as the GEMM's B operand)."""
 

@@ -32,10 +32,10 @@ from . import nn as F_ops
 _I, _L, _P = N.I, N.L, N.P
 N.register_optional("kfb_ssm_max_states", [])
 N.register_optional("kfb_ssm_floats", [_I] * 5, _L)
-N.register_optional("kfb_ssm_scan_fwd", [_I, _I] + [_P, _L] * 5 + [_P] * 9 + [_I] * 6 + [_P])
+N.register_optional("kfb_ssm_scan_fwd", [_I, _I] + [_P, _L] * 5 + [_P] * 9 + [_I] * 7 + [_P])
 N.register_optional("kfb_ssm_scan_bwd", [_I, _I] + [_P, _L] * 4 + [_P] * 16 + [_I] * 3 + [_P] +
-                    [_I] * 6 + [_P])
-N.register_optional("kfb_ssm_step", [_I] + [_P, _L] * 5 + [_P] * 5 + [_I] * 4 + [_P])
+                    [_I] * 7 + [_P])
+N.register_optional("kfb_ssm_step", [_I] + [_P, _L] * 5 + [_P] * 5 + [_I] * 5 + [_P])
 N.register_optional("kfb_cconv_max_taps", [])
 N.register_optional("kfb_cconv_bwd_ws", [_I] * 4, _L)
 N.register_optional("kfb_cconv_fwd", [_I, _I, _P, _L] + [_P] * 6 + [_I] * 6 + [_P])
@@ -279,8 +279,10 @@ def causal_conv_step(x, state, w, b=None, activation=None):
 
 # -------------------------------------------------------------- selective scan
 def selective_scan_reference(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=True,
-                             lengths=None, initial_state=None, reverse=False):
+                             lengths=None, initial_state=None, reverse=False, log_A=False):
     """Plain PyTorch (y, state) in A's precision: the oracle of the kernels."""
+    if log_A:
+        A = -torch.exp(A)
     T, Bn, Dn = x.shape
     pos, inside, _ = _positions(x, lengths, reverse)
     zero = torch.zeros((), dtype=A.dtype, device=x.device)
@@ -308,7 +310,8 @@ def selective_scan_reference(x, delta, A, B, C, D=None, z=None, delta_bias=None,
     return _take(y, pos).to(x.dtype), h
 
 
-def _scan_forward(x, delta, A, B, C, D, z, bias, lengths, h0, softplus, reverse, state, train):
+def _scan_forward(x, delta, A, B, C, D, z, bias, lengths, h0, softplus, reverse, log_A, state,
+                  train):
     T, Bn, Dn = x.shape
     Ns, dev = A.shape[0], x.device
     (x, ldx), (delta, ldd), (B, ldb), (C, ldc) = _rows(x), _rows(delta), _rows(B), _rows(C)
@@ -322,17 +325,17 @@ def _scan_forward(x, delta, A, B, C, D, z, bias, lengths, h0, softplus, reverse,
     N.call("kfb_ssm_scan_fwd", N.dt(x), V, x.data_ptr(), ldx, delta.data_ptr(), ldd, N.ptr(z), ldz,
            B.data_ptr(), ldb, C.data_ptr(), ldc, A.data_ptr(), N.ptr(D), N.ptr(bias),
            N.ptr(lengths), N.ptr(h0), N.ptr(hT), N.ptr(hs), bc.data_ptr(), y.data_ptr(), T, Bn, Dn,
-           Ns, int(softplus), int(reverse), N.stream(dev))
+           Ns, int(softplus), int(reverse), int(log_A), N.stream(dev))
     return y, hT, bc, hs
 
 
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, delta, A, B, C, D, z, bias, h0, lengths, softplus, reverse, state):
+    def forward(ctx, x, delta, A, B, C, D, z, bias, h0, lengths, softplus, reverse, log_A, state):
         y, hT, bc, hs = _scan_forward(x, delta, A, B, C, D, z, bias, lengths, h0, softplus,
-                                      reverse, state, True)
+                                      reverse, log_A, state, True)
         ctx.save_for_backward(x, delta, A, D, z, bias, lengths, bc, hs)
-        ctx.args = (softplus, reverse, h0 is not None)
+        ctx.args = (softplus, reverse, log_A, h0 is not None)
         ctx.params = (A, D, bias)
         ctx.set_materialize_grads(False)
         return (y, hT) if state else y
@@ -341,7 +344,7 @@ class _SelectiveScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dhT=None):
         x, delta, A, D, z, bias, lengths, bc, hs = ctx.saved_tensors
-        softplus, reverse, has_h0 = ctx.args
+        softplus, reverse, log_A, has_h0 = ctx.args
         T, Bn, Dn = x.shape
         Ns, dev, dt = A.shape[0], x.device, x.dtype
         if dy is None:
@@ -362,9 +365,9 @@ class _SelectiveScan(torch.autograd.Function):
                N.ptr(lengths), hs.data_ptr(), bc.data_ptr(), N.ptr(dhT), N.ptr(dh0), dx.data_ptr(),
                ddelta.data_ptr(), N.ptr(dz), dB.data_ptr(), dC.data_ptr(), N.ptr(grads[0]),
                N.ptr(grads[1]), N.ptr(grads[2]), acc[0], acc[1], acc[2], ws.data_ptr(), T, Bn, Dn,
-               Ns, int(softplus), int(reverse), N.stream(dev))
+               Ns, int(softplus), int(reverse), int(log_A), N.stream(dev))
         dA, dD, dbias = _grads_out(ctx.params, grads, acc)
-        return dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None
+        return dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None, None
 
 
 def _check_scan(x, delta, A, B, C, D, z, bias):
@@ -384,7 +387,7 @@ def _check_state(x, B, n, Dn, **states):
 
 
 def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=True, lengths=None,
-                   initial_state=None, return_state=False, reverse=False):
+                   initial_state=None, return_state=False, reverse=False, log_A=False):
     """The selective scan of x [T, B, D] with step sizes ``delta`` [T, B, D], input
     and output maps B, C [T, B, N] (all of one type) and decays A [N, D] (N = 1..64):
 
@@ -393,7 +396,8 @@ def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
         y   = (sum_n C_t h_t + D x) silu(z)
 
     A, D [D], delta_bias [D] fp32; D, z, delta_bias may be None.  dt A is meant to be
-    finite and not positive.  ``initial_state``: h before the first row (zero if
+    finite and not positive; ``log_A``: A is given as log(-A), the form that training
+    keeps negative (its gradient is that of the logarithm).  ``initial_state``: h before the first row (zero if
     None); ``return_state``: also h after each sequence's last row, from which
     selective_scan or selective_scan_step goes on.  Differentiable once in every
     tensor but ``lengths``."""
@@ -411,7 +415,7 @@ def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     _check_state(x, Bn, A.shape[0], Dn, initial_state=initial_state)
     if not x.is_cuda:
         y, h = selective_scan_reference(x, delta, A, B, C, D, z, delta_bias, softplus, lengths,
-                                        initial_state, reverse)
+                                        initial_state, reverse, log_A)
         return (y, h) if return_state else y
     N.dt(x)
     if Bn > 65535:
@@ -419,13 +423,15 @@ def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
     with F_ops.on_device(x):
         if _needs_grad(x, delta, A, B, C, D, z, delta_bias, initial_state):
             return _SelectiveScan.apply(x, delta, A, B, C, D, z, delta_bias, initial_state, lengths,
-                                        bool(softplus), bool(reverse), bool(return_state))
+                                        bool(softplus), bool(reverse), bool(log_A),
+                                        bool(return_state))
         y, h, _, _ = _scan_forward(x, delta, A, B, C, D, z, delta_bias, lengths, initial_state,
-                                   softplus, reverse, return_state, False)
+                                   softplus, reverse, log_A, return_state, False)
         return (y, h) if return_state else y
 
 
-def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=None, softplus=True):
+def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=None, softplus=True,
+                        log_A=False):
     """One token: x, delta, z [B, D], B, C [B, N] after ``state`` [B, N, D] (fp32,
     contiguous), which is moved on in place: y [B, D].  No gradient."""
     if x.dim() != 2 or x.numel() == 0:
@@ -451,7 +457,7 @@ def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     if not x.is_cuda:
         y, h = selective_scan_reference(x[None], delta[None], A, B[None], C[None], D,
                                         z[None] if z is not None else None, delta_bias, softplus,
-                                        None, state)
+                                        None, state, False, log_A)
         state.copy_(h)
         return y[0]
     (x, ldx), (delta, ldd), (B, ldb), (C, ldc) = _rows2(x), _rows2(delta), _rows2(B), _rows2(C)
@@ -460,5 +466,73 @@ def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     with F_ops.on_device(x):
         N.call("kfb_ssm_step", N.dt(x), x.data_ptr(), ldx, delta.data_ptr(), ldd, N.ptr(z), ldz,
                B.data_ptr(), ldb, C.data_ptr(), ldc, A.data_ptr(), N.ptr(D), N.ptr(delta_bias),
-               state.data_ptr(), y.data_ptr(), Bn, Dn, Ns, int(softplus), N.stream(dev))
+               state.data_ptr(), y.data_ptr(), Bn, Dn, Ns, int(softplus), int(log_A), N.stream(dev))
     return y
+
+
+# ----------------------------------------------------------------------- layer
+class _SplitColumns(torch.autograd.Function):
+    """Column slices of x [..., C], read in place; the backward puts their
+    gradients side by side in one native launch."""
+
+    @staticmethod
+    def forward(ctx, x, widths):
+        ctx.shape, ctx.widths = x.shape, widths
+        ctx.set_materialize_grads(False)
+        out, at = [], 0
+        for w in widths:
+            out.append(x[..., at:at + w])
+            at += w
+        return tuple(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        offs = [0]
+        for w in ctx.widths:
+            offs.append(offs[-1] + w)
+        some = next(g for g in grads if g is not None)
+        dx = some.new_empty(ctx.shape)
+        F_ops._concat_call(dx, [g.contiguous() if g is not None else None for g in grads], offs,
+                           dx.numel() // offs[-1], split=False)
+        return dx, None
+
+
+def split_columns(x, widths):
+    """x [..., sum(widths)] as slices of its last dim (GPU: no copy forward, one
+    native concatenation of the gradients backward)."""
+    if sum(widths) != x.shape[-1]:
+        raise ValueError("split_columns: %d columns do not split into %s" % (x.shape[-1],
+                                                                           tuple(widths)))
+    if not x.is_cuda or not x.requires_grad:
+        return torch.split(x, list(widths), dim=-1)
+    return _SplitColumns.apply(x.contiguous(), tuple(widths))
+
+
+def ssm_layer(x, w_in, conv_w, conv_b, w_rank, w_delta, w_bc, delta_bias, A_log, D, norm_w,
+              groups=1, lengths=None, reverse=False, low=None):
+    """One selective state space layer of x [T, B, din] -> [T, B, E]:
+
+        u, z = x w_in;  u = silu(causal_conv(u))
+        delta = u w_rank w_delta;  B, C = u w_bc
+        y = group_norm(selective_scan(u, delta, -exp(A_log), B, C, D, z), groups of a row)
+
+    w_in [din, 2 E], conv_w [K, E], w_rank [E, R], w_delta [R, E], w_bc [E, 2 N], A_log
+    [N, E] (fp32 masters in the TF layout); ``low``: compute-type copies of the
+    four matrices by name."""
+    T, B, din = x.shape
+    E, Ns = conv_w.shape[1], A_log.shape[0]
+    low = low or {}
+
+    def matmul(t, w, name):
+        return F_ops.linear(t, w, None, w_lp=low.get(name))
+
+    u, z = split_columns(matmul(x.reshape(T * B, din), w_in, "w_in").view(T, B, 2 * E), (E, E))
+    u = causal_conv(u, conv_w, conv_b, "silu", lengths, reverse=reverse)
+    # read by three consumers: their gradients are summed natively
+    us, ur, ub = F_ops.fanout(u, 3)
+    delta = matmul(matmul(ur.reshape(T * B, E), w_rank, "w_rank"), w_delta, "w_delta")
+    Bm, C = split_columns(matmul(ub.reshape(T * B, E), w_bc, "w_bc").view(T, B, 2 * Ns), (Ns, Ns))
+    y = selective_scan(us, delta.view(T, B, E), A_log, Bm, C, D, z, delta_bias, lengths=lengths,
+                       reverse=reverse, log_A=True)
+    return F_ops.group_norm(y.view(T * B, E), norm_w, None, groups).view(T, B, E)

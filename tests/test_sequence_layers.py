@@ -1,0 +1,400 @@
+"""The sequence and normalisation operators together, as models use them: the
+selective state space layer (ops.ssm.ssm_layer), DeepSpeech2 on it, group norm in
+the layer DSL, and the operators inside graphs, launch tapes and streams.
+
+Tolerances of comparisons between fp32 runs on two devices: each of the layer's
+eight operators rounds sums of up to n = 256 products, a relative error of about
+sqrt(n) 2^-24 = 1e-6 of its result's norm, and neither the norms nor the gates
+amplify by more than ten: 1e-4 for the chain.
+"""
+
+import pytest
+import torch
+
+from kf_benchmarks_amd.ops import nn as F
+from kf_benchmarks_amd.ops import ssm
+
+LAYER = ("w_in", "conv_w", "conv_b", "w_rank", "w_delta", "w_bc", "delta_bias", "A_log", "D", "norm_w")
+
+
+def relerr(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).norm() / b.norm())
+
+
+def layer_params(din, E, N=16, K=4, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    R = max(1, E // 16)
+    return {"w_in": r(din, 2 * E) / din ** 0.5, "conv_w": r(K, E) / K ** 0.5, "conv_b": 0.1 * r(E),
+            "w_rank": r(E, R) / E ** 0.5, "w_delta": r(R, E) / R ** 0.5, "w_bc": r(E, 2 * N) / E ** 0.5,
+            "delta_bias": r(E) - 3, "A_log": torch.log(1 + 3 * torch.rand(N, E, generator=g)), "D": r(E),
+            "norm_w": 1 + 0.1 * r(E)}
+
+
+def run_layer(x, p, dy=None, **kw):
+    x = x.detach().requires_grad_(dy is not None)
+    p = {k: v.detach().requires_grad_(dy is not None) for k, v in p.items()}
+    y = ssm.ssm_layer(x, **p, groups=4, **kw)
+    if dy is None:
+        return y
+    return [y] + list(torch.autograd.grad(y, [x] + [p[k] for k in LAYER], dy))
+
+
+# ------------------------------------------------------------------------- CPU
+def test_layer_cpu_padding_does_not_count():
+    """A padded batch gives what each sequence alone gives, in both directions."""
+    p = layer_params(12, 16)
+    x = torch.randn(9, 3, 12)
+    lengths = torch.tensor([9, 4, 1], dtype=torch.int32)
+    for reverse in (False, True):
+        y = run_layer(x, p, lengths=lengths, reverse=reverse)
+        for b, n in enumerate(lengths.tolist()):
+            alone = run_layer(x[:n, b:b + 1], p, reverse=reverse)
+            torch.testing.assert_close(y[:n, b:b + 1], alone, rtol=1e-4, atol=1e-5)
+
+
+def test_split_columns():
+    x = torch.randn(3, 2, 7, requires_grad=True)
+    a, b = ssm.split_columns(x, (3, 4))
+    (a.sum() + 2 * b.sum()).backward()
+    assert torch.equal(x.grad, torch.cat([torch.ones(3, 2, 3), torch.full((3, 2, 4), 2.0)], -1))
+    with pytest.raises(ValueError):
+        ssm.split_columns(x, (3, 3))
+
+
+def _norm_net(device, dtype):
+    """A small residual net in the layer DSL, its norms group norms."""
+    from kf_benchmarks_amd import params as P
+    from kf_benchmarks_amd.models.model import CNNModel, Network
+
+    class Net(CNNModel):
+        def __init__(self, params=None):
+            super().__init__("gnnet", 16, 4, 0.01, params=params)
+
+        def add_inference(self, cnn):
+            cnn.conv(16, 3, 3, 1, 1, activation=None, bias=None)
+            a = cnn.group_norm(4, activation="relu")
+            cnn.conv(16, 3, 3, 1, 1, activation=None, bias=None)
+            cnn.group_norm(8, activation="silu")
+            cnn.add(cnn.top_layer, a)
+            cnn.spatial_mean()
+
+    torch.manual_seed(0)
+    return Network(Net(P.make_params(model="trivial")), 10, device, dtype)
+
+
+def _norm_net_run(net, images):
+    logits = net.forward_inputs([images])
+    logits = getattr(logits, "logits", logits)
+    if isinstance(logits, (tuple, list)):
+        logits = logits[0]
+    net.zero_grad()
+    (logits.float() ** 2).sum().backward()
+    return logits, {n: p.grad for n, p in net.named_parameters()}
+
+
+def test_group_norm_in_the_layer_dsl_cpu():
+    net = _norm_net("cpu", torch.float32)
+    names = set(net.tf_variables())
+    assert "v0/cg/groupnorm0/gamma" in names and "v0/cg/groupnorm1/beta" in names
+    logits, grads = _norm_net_run(net, torch.randn(2, 16, 16, 3))
+    assert logits.shape == (2, 10) and all(g is not None and torch.isfinite(g).all() for g in grads.values())
+
+
+def test_deepspeech2_ssm_cpu():
+    from kf_benchmarks_amd.models.deepspeech import DeepSpeech2Model
+    with pytest.raises(ValueError):
+        DeepSpeech2Model(rnn_type="ssn")
+    assert "ssm" in DeepSpeech2Model.SUPPORTED_RNNS
+
+
+# ------------------------------------------------------------------------- GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{}, {"reverse": True}, {"ragged": True}])
+def test_layer_gpu_matches_cpu(cuda, kw):
+    kw = dict(kw)
+    T, B, din, E = 40, 4, 48, 64
+    p = layer_params(din, E)
+    x, dy = torch.randn(T, B, din), torch.randn(T, B, E)
+    lengths = torch.tensor([40, 3, 17, 0], dtype=torch.int32) if kw.pop("ragged", False) else None
+    want = run_layer(x, p, dy, lengths=lengths, **kw)
+    got = run_layer(x.to(cuda), {k: v.to(cuda) for k, v in p.items()}, dy.to(cuda),
+                    lengths=lengths.to(cuda) if lengths is not None else None, **kw)
+    for name, a, b in zip(("y", "x") + LAYER, got, want):
+        assert relerr(a, b) < 1e-4, (name, relerr(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_token_by_token_gpu(cuda, dtype):
+    """A prompt through the layer's operators, then single tokens: the outputs of
+    the whole sequence at once (bf16: each intermediate of the tokens is rounded as the
+    sequence's is, but their sums are not the same: two roundings each)."""
+    T, B, E, N, K, P = 12, 3, 64, 16, 4, 7
+    p = {k: v.to(cuda) for k, v in layer_params(E, E, N, K).items()}
+    low = {k: p[k].to(dtype) for k in ("w_in", "w_rank", "w_delta", "w_bc")}
+    x = torch.randn(T, B, E, device=cuda).to(dtype)
+
+    def token(u, z, state):
+        u = ssm.causal_conv_step(u, state[0], p["conv_w"], p["conv_b"], "silu")
+        delta = F.linear(F.linear(u, p["w_rank"], None, low["w_rank"]), p["w_delta"], None, low["w_delta"])
+        bc = F.linear(u, p["w_bc"], None, low["w_bc"])
+        y = ssm.selective_scan_step(u, delta, p["A_log"], bc[:, :N], bc[:, N:], state[1], p["D"], z, p["delta_bias"],
+                                    log_A=True)
+        return F.group_norm(y, p["norm_w"], None, 4)
+
+    with torch.no_grad():
+        want = ssm.ssm_layer(x, **p, groups=4, low=low)
+        xz = F.linear(x.view(T * B, E), p["w_in"], None, low["w_in"]).view(T, B, 2 * E)
+        u, last = ssm.causal_conv(xz[:P, :, :E], p["conv_w"], p["conv_b"], "silu", return_state=True)
+        delta = F.linear(F.linear(u.view(P * B, E), p["w_rank"], None, low["w_rank"]), p["w_delta"], None, low["w_delta"])
+        bc = F.linear(u.view(P * B, E), p["w_bc"], None, low["w_bc"]).view(P, B, 2 * N)
+        y, h = ssm.selective_scan(u, delta.view(P, B, E), p["A_log"], bc[..., :N], bc[..., N:], p["D"], xz[:P, :, E:],
+                                  p["delta_bias"], return_state=True, log_A=True)
+        got = [F.group_norm(y.view(P * B, E), p["norm_w"], None, 4).view(P, B, E)]
+        state = (last, h)
+        for t in range(P, T):
+            got.append(token(xz[t, :, :E], xz[t, :, E:], state)[None])
+    assert relerr(torch.cat(got), want) < (1e-4 if dtype == torch.float32 else 2 ** -6)
+
+
+@pytest.mark.gpu
+def test_group_norm_in_the_layer_dsl_gpu(cuda):
+    a, b = _norm_net("cpu", torch.float32), _norm_net(str(cuda), torch.float32)
+    b.load_state_dict(a.state_dict())
+    images = torch.randn(2, 16, 16, 3)
+    la, ga = _norm_net_run(a, images)
+    lb, gb = _norm_net_run(b, images.to(cuda))
+    assert relerr(lb, la) < 1e-4
+    for n in ga:
+        assert relerr(gb[n], ga[n]) < 1e-3, n  # the convolutions' backward sums 512 products a weight
+
+
+@pytest.mark.gpu
+def test_deepspeech2_ssm_gpu_matches_cpu(cuda):
+    from kf_benchmarks_amd import datasets, params as P
+    from kf_benchmarks_amd.models import model_config
+    from kf_benchmarks_amd.models.model import make_network
+    d = datasets.create_dataset(None, "librispeech")
+    losses, grads, inputs = [], [], None
+    for dev in ("cpu", cuda):
+        m = model_config.get_model_config("deepspeech2", d, P.make_params(model="deepspeech2"))
+        m.max_time_steps, m.max_label_length, m.rnn_hidden_size, m.num_rnn_layers = 120, 20, 32, 2
+        m.rnn_type = "ssm"
+        m.set_batch_size(4)
+        torch.manual_seed(0)
+        net = make_network(m, d.num_classes, str(dev), torch.float32)
+        if inputs is None:
+            inputs = m.get_synthetic_inputs("x", d.num_classes, "cpu", 0)
+        inp = tuple(t.to(dev) for t in inputs)
+        loss = m.loss_function(inp, net.forward_inputs(inp))
+        loss.backward()
+        losses.append(float(loss))
+        grads.append(torch.cat([p.grad.reshape(-1).float().cpu() for p in net.parameters() if p.grad is not None]))
+        assert any(n.endswith("A_log_0") for n, p in net.named_parameters() if p.grad is not None)
+    assert abs(losses[0] - losses[1]) < 1e-3 * abs(losses[0])
+    assert relerr(grads[1], grads[0]) < 1e-2  # as the recurrent layers' test: the batch norms amplify
+
+
+@pytest.mark.gpu
+def test_deepspeech2_ssm_with_launch_tape_gpu(cuda, monkeypatch):
+    """The step is made only of native calls, so it is recorded and replayed."""
+    from kf_benchmarks_amd import params as P
+    from kf_benchmarks_amd.benchmark import BenchmarkCNN
+    monkeypatch.setenv("KFB_TAPE_STRICT", "1")
+    runs = []
+    for tape in (True, False):
+        b = BenchmarkCNN(P.make_params(model="deepspeech2", batch_size=2, num_gpus=1, use_bf16=True, optimizer="momentum",
+                                       data_format="NHWC", variable_update="kungfu", launch_tape=tape,
+                                       init_learning_rate=1e-4, display_every=10 ** 9, data_name="librispeech"))
+        b.model.rnn_type, b.model.num_rnn_layers = "ssm", 2
+        b.build()
+        runs.append((b, [float(b.train_step(need_loss=True)[0]) for _ in range(5)]))
+        torch.cuda.synchronize()
+    (bt, lt), (_, le) = runs
+    assert getattr(bt, "_tape", None) is not None, getattr(bt, "_tape_reason", None)
+    for a, b in zip(lt, le):
+        assert abs(a - b) <= 0.02 * max(1.0, abs(b)), (lt, le)
+
+
+def _all_ops(x, c, step_states):
+    """Every operator once, forward and backward: a list of tensors."""
+    outs = []
+    gx = x["img"].detach().requires_grad_()
+    gamma = c["gamma"].detach().requires_grad_()
+    y = F.group_norm(gx, gamma, c["beta"], 8, activation="silu")
+    outs += [y, *torch.autograd.grad(y, (gx, gamma), x["dimg"])]
+    big = x["big"].detach().requires_grad_()
+    y = F.group_norm(big, c["gamma"], c["beta"], 8, activation="relu")
+    outs += [y, *torch.autograd.grad(y, (big,), big.detach())]
+    sx = x["seq"].detach().requires_grad_()
+    w = c["w"].detach().requires_grad_()
+    u = ssm.causal_conv(sx, w, c["b"], "silu")
+    A = c["A"].detach().requires_grad_()
+    y, h = ssm.selective_scan(u, x["delta"], A, x["B"], x["C"], c["D"], x["z"], c["bias"], return_state=True)
+    outs += [u, y, h, *torch.autograd.grad((y, h), (sx, w, A), (x["dseq"], torch.ones_like(h)))]
+    with torch.no_grad():
+        outs.append(ssm.causal_conv_step(x["seq"][0], step_states[0], c["w"], c["b"], "silu"))
+        outs.append(ssm.selective_scan_step(x["seq"][0], x["delta"][0], c["A"], x["B"][0], x["C"][0], step_states[1], c["D"],
+                                            x["z"][0], c["bias"]))
+    return [t.detach() for t in outs]
+
+
+def _all_inputs(dev, seed, T=200, B=2, D=96, N=16):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    bf = torch.bfloat16
+    x = {"img": r(3, 7, 7, 64).to(bf), "dimg": r(3, 7, 7, 64).to(bf), "big": r(2, 90, 90, 64).to(bf), "seq": r(T, B, D).to(bf),
+         "delta": r(T, B, D).to(bf), "B": r(T, B, N).to(bf), "C": r(T, B, N).to(bf), "z": r(T, B, D).to(bf), "dseq": r(T, B, D).to(bf)}
+    c = {"gamma": r(64), "beta": r(64), "w": r(4, D), "b": r(D), "A": -r(N, D).abs() - 0.1, "D": r(D), "bias": r(D) - 2}
+    return x, c, (r(3, B, D).to(bf), r(B, N, D))
+
+
+@pytest.mark.gpu
+def test_inside_graphs_gpu(cuda):
+    """Forward and backward of every operator captured, in two graphs that share a memory pool: replays on new
+    inputs, with eager work between them, give the eager bits."""
+    x, c, _ = _all_inputs(cuda, 0)
+    states = [tuple(torch.zeros_like(s) for s in _all_inputs(cuda, 0)[2]) for _ in range(3)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _all_ops(x, c, states[2])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs, pool = [], [], None
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(_all_ops(x, c, states[k]))
+        pool = g.pool()
+        graphs.append(g)
+    for seed in (1, 2, 3):
+        fresh, _, start = _all_inputs(cuda, seed)
+        for k in x:
+            x[k].copy_(fresh[k])
+        for k in (0, 1, 0):
+            for s, v in zip(states[k], start):
+                s.copy_(v)
+            eager_states = tuple(v.clone() for v in start)
+            want = _all_ops(x, c, eager_states)
+            graphs[k].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs[k], want))
+            assert all(torch.equal(a, b) for a, b in zip(states[k], eager_states))
+
+
+@pytest.mark.gpu
+def test_inside_a_launch_tape_gpu(cuda):
+    """Recorded by the step executor and replayed from C++ on other inputs."""
+    from kf_benchmarks_amd.ops import _native as N
+    from kf_benchmarks_amd.ops.tape import StepTape
+    x, c, start = _all_inputs(cuda, 0)
+    dh = torch.ones(2, 16, 96, device=cuda)
+    state = tuple(s.clone() for s in start)
+
+    def step():
+        gx = x["img"].detach().requires_grad_()
+        y = F.group_norm(gx, c["gamma"], c["beta"], 8, activation="silu")
+        outs = [y, *torch.autograd.grad(y, (gx,), x["dimg"])]
+        sx = x["seq"].detach().requires_grad_()
+        u = ssm.causal_conv(sx, c["w"], c["b"], "silu")
+        A = c["A"].detach().requires_grad_()
+        y, h = ssm.selective_scan(u, x["delta"], A, x["B"], x["C"], c["D"], x["z"], c["bias"], return_state=True)
+        outs += [u, y, h, *torch.autograd.grad((y, h), (sx, A), (x["dseq"], dh))]
+        with torch.no_grad():
+            outs.append(ssm.causal_conv_step(x["seq"][0], state[0], c["w"], c["b"], "silu"))
+            outs.append(ssm.selective_scan_step(x["seq"][0], x["delta"][0], c["A"], x["B"][0], x["C"][0], state[1],
+                                                c["D"], x["z"][0], c["bias"]))
+        return [t.detach() for t in outs]
+
+    tape = StepTape(cuda)
+    outs = tape.record(step)
+    assert not N.recording()
+    for seed in (1, 2):
+        fresh, _, begin = _all_inputs(cuda, seed)
+        for k in x:
+            x[k].copy_(fresh[k])
+        for s, v in zip(state, begin):
+            s.copy_(v)
+        torch.cuda.synchronize()
+        tape.replay({})
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs]
+        for s, v in zip(state, begin):
+            s.copy_(v)
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+    tape.close()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once_gpu(cuda):
+    """The same calls on two streams at the same time, many times over: neither sees the other's workspace."""
+    sets = [_all_inputs(cuda, s) for s in (4, 5)]
+    want = [_all_ops(x, c, tuple(t.clone() for t in st)) for x, c, st in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for k, (x, c, st) in enumerate(sets):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(_all_ops(x, c, tuple(t.clone() for t in st)))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for run in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[k]))
+
+
+@pytest.mark.gpu
+def test_long_offsets_gpu(cuda):
+    """More than 2^31 values in a tensor: the second half of a sequence, run alone from the first half's state,
+    gives the same (to a rounding of the result: the chunks fall differently)."""
+    T, D, N = 1 << 20, 2304, 2
+    x = torch.randn(4096, 1, D, device=cuda).to(torch.bfloat16).repeat(T // 4096, 1, 1)
+    assert x.numel() > 2 ** 31
+    w, A = torch.randn(2, D, device=cuda), -torch.rand(N, D, device=cuda) - 0.5
+    bc = torch.randn(T, 1, 2 * N, device=cuda).to(torch.bfloat16)
+    h = T // 2
+    with torch.no_grad():
+        y, last = ssm.causal_conv(x, w, return_state=True)
+        ya, s = ssm.causal_conv(x[:h], w, return_state=True)
+        yb, lb = ssm.causal_conv(x[h:], w, initial_state=s, return_state=True)
+        assert torch.equal(y[:h], ya) and torch.equal(y[h:], yb) and torch.equal(last, lb)
+        del ya, yb
+        dt = y.abs_()
+        y, last = ssm.selective_scan(x, dt, A, bc[..., :N], bc[..., N:], softplus=False, return_state=True)
+        _, s = ssm.selective_scan(x[:h], dt[:h], A, bc[:h, :, :N], bc[:h, :, N:], softplus=False, return_state=True)
+        yb, lb = ssm.selective_scan(x[h:], dt[h:], A, bc[h:, :, :N], bc[h:, :, N:], softplus=False, initial_state=s,
+                                    return_state=True)
+    torch.testing.assert_close(last, lb, rtol=1e-5, atol=1e-5)
+    for a in range(0, h, h // 8):
+        p, q = y[h + a:h + a + 512].float(), yb[a:a + 512].float()
+        assert ((p - q).abs() <= 2 ** -7 * p.abs() + 1e-4).all()
+    assert torch.isfinite(y[-512:].float()).all()
+
+
+@pytest.mark.gpu
+def test_no_second_derivatives_gpu(cuda):
+    x, c, _ = _all_inputs(cuda, 0)
+    sx = x["seq"].detach().requires_grad_()
+    for y in (ssm.causal_conv(sx, c["w"]), ssm.selective_scan(sx, x["delta"], c["A"], x["B"], x["C"])):
+        (g,) = torch.autograd.grad(y.float().sum(), sx, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.float().sum().backward()
+
+
+@pytest.mark.gpu
+def test_gradient_of_the_state_alone_gpu(cuda):
+    """Only the returned state is used: its gradient alone flows back."""
+    x, c, _ = _all_inputs(cuda, 0, T=20)
+    grads = []
+    for dev in ("cpu", cuda):
+        sx = x["seq"].to(dev).float().requires_grad_()
+        f = lambda t: t.to(dev).float()  # noqa: E731
+        _, s = ssm.causal_conv(sx, f(c["w"]), return_state=True)
+        _, h = ssm.selective_scan(sx, f(x["delta"]), f(c["A"]), f(x["B"]), f(x["C"]), return_state=True)
+        grads.append(torch.autograd.grad(s.sum() + h.sum(), sx)[0])
+    assert relerr(grads[1], grads[0]) < 1e-5

@@ -51,7 +51,7 @@ def scan_oracle(i, dy=None, dh=None, size=False):
         return torch.where(inside, gather(t.double(), pos), zero)
 
     x, Bm, C = (mag(take(i[k])) for k in ("x", "B", "C"))
-    A = i["A"].double()
+    A = -torch.exp(i["A"].double()) if i.get("log_A") else i["A"].double()
     raw = take(i["delta"]) + (i["bias"].double() if i["bias"] is not None else 0)
     dt = torch.where(inside, raw.clamp(min=0) + torch.log1p(torch.exp(-raw.abs())) if i["softplus"] else raw, zero)
     slope = torch.sigmoid(raw) if i["softplus"] else torch.ones_like(raw)
@@ -85,7 +85,7 @@ def scan_oracle(i, dy=None, dh=None, size=False):
         dC[t] = (e[t][:, None] * after[t]).sum(2)
         carry = g * a[t]
     dd = torch.stack(dd) * slope
-    out |= {"x": inv(torch.stack(dx)), "delta": inv(dd), "A": dA, "B": inv(torch.stack(dB)),
+    out |= {"x": inv(torch.stack(dx)), "delta": inv(dd), "A": dA * mag(A) if i.get("log_A") else dA, "B": inv(torch.stack(dB)),
             "C": inv(torch.stack(dC)), "D": (e * x).sum((0, 1)), "bias": torch.where(inside, dd, zero).sum((0, 1)), "state": carry}
     if z is not None:
         # silu'(z) = p (1 + z (1 - p)) cancels at z = -1.278: the magnitudes on the way are p (1 + |z| (1 - p)),
@@ -151,7 +151,7 @@ def check(got, value, bound, name):
 
 
 def scan_inputs(T, B, D, n, dtype, dev, seed=0, z=True, skip=True, bias=True, softplus=True, ragged=False,
-                state=False, reverse=False, slices=False, poison=False):
+                state=False, reverse=False, slices=False, poison=False, log_A=False):
     g = torch.Generator().manual_seed(seed)
 
     def rand(*s):
@@ -176,7 +176,9 @@ def scan_inputs(T, B, D, n, dtype, dev, seed=0, z=True, skip=True, bias=True, so
         i = {k: t.contiguous() if t is not None else None for k, t in i.items()}
     i |= {"A": -(0.2 + 2 * torch.rand(n, D, generator=g)).to(dev), "D": rand(D).to(dev) if skip else None,
           "bias": (rand(D) - 1).to(dev) if bias and softplus else None, "state": rand(B, n, D).to(dev) if state else None}
-    i |= {"lengths": lengths.to(dev) if ragged else None, "softplus": softplus, "reverse": reverse}
+    i |= {"lengths": lengths.to(dev) if ragged else None, "softplus": softplus, "reverse": reverse, "log_A": log_A}
+    if log_A:
+        i["A"] = torch.log(-i["A"])
     dy, dh = rand(T, B, D).to(dtype).to(dev), rand(B, n, D).to(dev)
     return i, dy, dh
 
@@ -190,7 +192,7 @@ def scan_run(i, dy=None, dh=None):
         for k in SCAN_LEAVES:
             i[k] = i[k].detach().requires_grad_() if i[k] is not None else None
     y, h = ssm.selective_scan(i["x"], i["delta"], i["A"], i["B"], i["C"], i["D"], i["z"], i["bias"], i["softplus"],
-                              i["lengths"], i["state"], True, i["reverse"])
+                              i["lengths"], i["state"], True, i["reverse"], i["log_A"])
     out = {"y": y.detach(), "state_out": h.detach()}
     if dy is not None:
         names = [k for k in SCAN_LEAVES if i[k] is not None]
@@ -268,9 +270,10 @@ def conv_compare(T, B, D, K, dtype, dev, state_grad=True, **kw):
 # ------------------------------------------------------------------------- CPU
 OPTIONS = [{}, {"ragged": True, "poison": True}, {"state": True}, {"reverse": True},
            {"ragged": True, "state": True, "reverse": True}]
+SCAN_OPTIONS = OPTIONS + [{"log_A": True}]
 
 
-@pytest.mark.parametrize("kw", OPTIONS)
+@pytest.mark.parametrize("kw", SCAN_OPTIONS)
 def test_selective_scan_cpu(kw):
     scan_compare(7, 4, 6, 3, torch.float32, "cpu", **kw)
 
@@ -297,7 +300,7 @@ def _differences(oracle, i, leaves, out_grads, kw):
             assert abs((f[0] - f[1]) / 2e-6 - want[name].reshape(-1)[j]) < 1e-6 * (1 + abs(want[name].reshape(-1)[j])), name
 
 
-@pytest.mark.parametrize("kw", OPTIONS[:1] + OPTIONS[2:] + [{"softplus": False}, {"z": False, "skip": False}])
+@pytest.mark.parametrize("kw", OPTIONS[:1] + OPTIONS[2:] + [{"softplus": False}, {"z": False, "skip": False}, {"log_A": True}])
 def test_scan_oracle_gradients_against_differences(kw):
     i, dy, dh = scan_inputs(5, 4, 3, 2, torch.float64, "cpu", **kw)
     i = {k: t.double() if torch.is_tensor(t) and t.is_floating_point() else t for k, t in i.items()}
@@ -406,7 +409,7 @@ def test_selective_scan_gpu(cuda, T, B, D, n, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("kw", OPTIONS + [{"z": False}, {"skip": False, "bias": False}, {"softplus": False},
+@pytest.mark.parametrize("kw", SCAN_OPTIONS + [{"z": False}, {"skip": False, "bias": False}, {"softplus": False},
                                           {"slices": True}, {"state_grad": False, "z": False}])
 @pytest.mark.parametrize("T,B,D,n", [(37, 4, 72, 16), (2, 3, 33, 6), (70, 4, 64, 40)])
 def test_selective_scan_options_gpu(cuda, T, B, D, n, kw):
