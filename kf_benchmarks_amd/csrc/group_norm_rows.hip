@@ -4,8 +4,11 @@
 // formulas are group_norm.hip's.
 //
 // Bound by HBM.  A set of L lanes keeps one group index g (gamma, beta and, in the
-// backward, the channel sums stay in registers) and walks over the rows, U of
-// them at a time so that U K loads are in flight.
+// backward, the channel sums stay in registers) and walks over the rows, the next
+// row loaded while one is worked on.  8192 waves, one row at a time: 22.2 us for
+// 13984 rows of 1600 bf16 values in 8 groups (4.0 TB/s; a copy reaches 5.2);
+// 4096 waves took 25.3 us, two rows at a time 25.1, 16384 waves (each reads gamma
+// and beta, as many bytes as its rows) 33.6.
 #include "group_norm.h"
 
 namespace kfb {
@@ -32,7 +35,6 @@ __device__ __forceinline__ float set_sum(float v, int L) {
 
 template <typename T, int V, int KIND, int K>
 __global__ void __launch_bounds__(RNT) gn_rows_fwd_k(Args a, Rows w) {
-  constexpr int U = K >= 4 ? 1 : 4 / K;
   const int set = (int)((blockIdx.x * RNT + threadIdx.x) / w.L), j = threadIdx.x % w.L;
   if (set >= w.sets) return;
   const int g = set % a.G, c0 = g * a.cpg;
@@ -46,68 +48,54 @@ __global__ void __launch_bounds__(RNT) gn_rows_fwd_k(Args a, Rows w) {
   const float inv = 1.f / (float)a.cpg;
   const T* __restrict__ x = (const T*)a.x + c0 + j * V;
   T* __restrict__ y = (T*)a.y + c0 + j * V;
-  for (long n0 = set / a.G; n0 < a.N; n0 += (long)U * w.slabs) {
-    Raw<T, V> raw[U][K];
-    float mu[U], rs[U];
+  Raw<T, V> next[K];
+  auto fetch = [&](long n) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long n = n0 + (long)u * w.slabs;
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        raw[u][k].zero();
-        if (n < a.N && j + k * w.L < w.nv) raw[u][k].load(x + n * a.C + (long)k * w.L * V);
-      }
+    for (int k = 0; k < K; ++k) {
+      next[k].zero();
+      if (j + k * w.L < w.nv) next[k].load(x + n * a.C + (long)k * w.L * V);
     }
+  };
+  long n = set / a.G;
+  if (n < a.N) fetch(n);
+  for (; n < a.N; n += w.slabs) {
+    Raw<T, V> raw[K];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float s = 0.f;
+    for (int k = 0; k < K; ++k) raw[k] = next[k];
+    if (n + w.slabs < a.N) fetch(n + w.slabs);  // while this row is worked on
+    float s = 0.f, m2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += raw[u][k][i];
-      mu[u] = s;
-    }
+      for (int i = 0; i < V; ++i) s += raw[k][i];
+    const float mu = set_sum(s, w.L) * inv;
 #pragma unroll
-    for (int u = 0; u < U; ++u) mu[u] = set_sum(mu[u], w.L) * inv;
+    for (int k = 0; k < K; ++k)
+      if (j + k * w.L < w.nv)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float s = 0.f;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (j + k * w.L < w.nv)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float d = raw[u][k][i] - mu[u];
-            s = fmaf(d, d, s);
-          }
-      rs[u] = s;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) rs[u] = 1.f / sqrtf(set_sum(rs[u], w.L) * inv + a.eps);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long n = n0 + (long)u * w.slabs;
-      if (n >= a.N) break;
-      if (j == 0) {
-        a.mean[n * a.G + g] = mu[u];
-        a.rstd[n * a.G + g] = rs[u];
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (j + k * w.L < w.nv) {
-          float o[V];
-#pragma unroll
-          for (int i = 0; i < V; ++i)
-            o[i] = act_fwd<KIND>(fmaf((raw[u][k][i] - mu[u]) * rs[u], ga[k][i], be[k][i]), a.act);
-          store_vec<T, V>(y + n * a.C + (long)k * w.L * V, o);
+        for (int i = 0; i < V; ++i) {
+          const float d = raw[k][i] - mu;
+          m2 = fmaf(d, d, m2);
         }
+    const float rs = 1.f / sqrtf(set_sum(m2, w.L) * inv + a.eps);
+    if (j == 0) {
+      a.mean[n * a.G + g] = mu;
+      a.rstd[n * a.G + g] = rs;
     }
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (j + k * w.L < w.nv) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          o[i] = act_fwd<KIND>(fmaf((raw[k][i] - mu) * rs, ga[k][i], be[k][i]), a.act);
+        store_vec<T, V>(y + n * a.C + (long)k * w.L * V, o);
+      }
   }
 }
 
 template <typename T, int V, int KIND, int K>
 __global__ void __launch_bounds__(RNT) gn_rows_bwd_k(Args a, Rows w) {
-  constexpr int U = K >= 2 ? 1 : 2;
   const int set = (int)((blockIdx.x * RNT + threadIdx.x) / w.L), j = threadIdx.x % w.L;
   if (set >= w.sets) return;
   const int g = set % a.G, c0 = g * a.cpg, slab = set / a.G;
@@ -124,62 +112,53 @@ __global__ void __launch_bounds__(RNT) gn_rows_bwd_k(Args a, Rows w) {
   const T* __restrict__ x = (const T*)a.x + c0 + j * V;
   const T* __restrict__ dy = (const T*)a.dy + c0 + j * V;
   T* __restrict__ dx = (T*)a.y + c0 + j * V;
-  for (long n0 = slab; n0 < a.N; n0 += (long)U * w.slabs) {
-    Raw<T, V> rx[U][K], rd[U][K];
-    float mu[U][1], rs[U][1], s1[U], s2[U];
+  Raw<T, V> nx[K], nd[K];
+  float nmu = 0.f, nrs = 0.f;
+  auto fetch = [&](long n) {
+    nmu = a.mean[n * a.G + g];
+    nrs = a.rstd[n * a.G + g];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long n = n0 + (long)u * w.slabs;
-      const bool on = n < a.N;
-      mu[u][0] = on ? a.mean[n * a.G + g] : 0.f;
-      rs[u][0] = on ? a.rstd[n * a.G + g] : 0.f;
+    for (int k = 0; k < K; ++k)
+      if (j + k * w.L < w.nv) {
+        nx[k].load(x + n * a.C + (long)k * w.L * V);
+        nd[k].load(dy + n * a.C + (long)k * w.L * V);
+      }
+  };
+  if (slab < a.N) fetch(slab);
+  for (long n = slab; n < a.N; n += w.slabs) {
+    Raw<T, V> rx[K], rd[K];
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        rx[u][k].zero();
-        rd[u][k].zero();
-        if (on && j + k * w.L < w.nv) {
-          rx[u][k].load(x + n * a.C + (long)k * w.L * V);
-          rd[u][k].load(dy + n * a.C + (long)k * w.L * V);
+    for (int k = 0; k < K; ++k) {
+      rx[k] = nx[k];
+      rd[k] = nd[k];
+    }
+    const float mu[1] = {nmu}, rs[1] = {nrs};
+    if (n + w.slabs < a.N) fetch(n + w.slabs);  // while this row is worked on
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (j + k * w.L < w.nv) {
+        float e[V], xh[V];
+        grad_terms<T, V, 1, KIND>(a, rx[k], rd[k], mu, rs, ga[k], be[k], e, xh);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          cp[k][i] += e[i];
+          cq[k][i] = fmaf(e[i], xh[i], cq[k][i]);
+          s1 = fmaf(ga[k][i], e[i], s1);
+          s2 = fmaf(ga[k][i] * e[i], xh[i], s2);
         }
       }
-    }
+    s1 = set_sum(s1, w.L) * inv;
+    s2 = set_sum(s2, w.L) * inv;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      s1[u] = s2[u] = 0.f;
-      if (n0 + (long)u * w.slabs >= a.N) continue;
+    for (int k = 0; k < K; ++k)
+      if (j + k * w.L < w.nv) {
+        float e[V], xh[V];
+        grad_terms<T, V, 1, KIND>(a, rx[k], rd[k], mu, rs, ga[k], be[k], e, xh);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (j + k * w.L < w.nv) {
-          float e[V], xh[V];
-          grad_terms<T, V, 1, KIND>(a, rx[u][k], rd[u][k], mu[u], rs[u], ga[k], be[k], e, xh);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            cp[k][i] += e[i];
-            cq[k][i] = fmaf(e[i], xh[i], cq[k][i]);
-            s1[u] = fmaf(ga[k][i], e[i], s1[u]);
-            s2[u] = fmaf(ga[k][i] * e[i], xh[i], s2[u]);
-          }
-        }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      s1[u] = set_sum(s1[u], w.L) * inv;
-      s2[u] = set_sum(s2[u], w.L) * inv;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long n = n0 + (long)u * w.slabs;
-      if (n >= a.N) break;
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-        if (j + k * w.L < w.nv) {
-          float e[V], xh[V];
-          grad_terms<T, V, 1, KIND>(a, rx[u][k], rd[u][k], mu[u], rs[u], ga[k], be[k], e, xh);
-#pragma unroll
-          for (int i = 0; i < V; ++i) e[i] = rs[u][0] * (fmaf(ga[k][i], e[i], -s1[u]) - xh[i] * s2[u]);
-          store_vec<T, V>(dx + n * a.C + (long)k * w.L * V, e);
-        }
-    }
+        for (int i = 0; i < V; ++i) e[i] = rs[0] * (fmaf(ga[k][i], e[i], -s1) - xh[i] * s2);
+        store_vec<T, V>(dx + n * a.C + (long)k * w.L * V, e);
+      }
   }
   float* out = a.part + (long)slab * 2 * a.C + c0 + j * V;
 #pragma unroll
@@ -193,14 +172,14 @@ __global__ void __launch_bounds__(RNT) gn_rows_bwd_k(Args a, Rows w) {
 }
 
 // Lane sets that fill the card and no more than the rows need.  Backward: each
-// slab of rows leaves 2 C sums to add up, so it has an eighth of the waves.
+// slab of rows leaves 2 C sums to add up, so it has half the waves.
 static Rows rows_of(long N, int C, int G, int V, bool bwd, int& K) {
   Rows w;
   w.nv = C / G / V;
   w.L = 1;
   while (w.L < 64 && w.L < w.nv) w.L *= 2;
   K = ceil_div(w.nv, w.L);
-  const long waves = bwd ? 4096 : 16384;
+  const long waves = bwd ? 4096 : 8192;
   long slabs = ceil_div(waves * 64 / w.L, G);
   const long most = bwd ? ceil_div(N, 4) : N;
   if (slabs > most) slabs = most;
