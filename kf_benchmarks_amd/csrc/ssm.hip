@@ -49,6 +49,7 @@ struct Args {
   float *ends, *sums;
   int nchunk, tpc;
   int T, B, D, N, W, Tp, softplus, reverse, log_a;
+  FastDiv by2n;
 };
 
 // B and C as constant memory: uniform addresses become scalar loads
@@ -82,10 +83,13 @@ __device__ __forceinline__ int seq_len(const Args& a, int b) {
   return a.len ? min(max(a.len[b], 0), a.T) : a.T;
 }
 
-// the row of position s
+// the time of position s
+__device__ __forceinline__ long time_of(const Args& a, int s, int len) {
+  return a.reverse && s < len ? len - 1 - s : s;
+}
+
 __device__ __forceinline__ long row_of(const Args& a, int b, int s, int len) {
-  const int t = a.reverse && s < len ? len - 1 - s : s;
-  return (long)t * a.B + b;
+  return time_of(a, s, len) * a.B + b;
 }
 
 // B and C in fp32, per wave, zero past a sequence's end and past N (a row that
@@ -248,6 +252,7 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
         put(sx + at, qx);
       }
   };
+  const long ystep = (long)a.B * a.D, ybase = (long)b * a.D + me.c;
   float sum_dt = 0.f;
   int s0 = chunk * a.tpc * TQ;
   Group<NS, UR> next;
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
             for (int k = 0; k < V; ++k) v[k] *= siluf(cz[i][k]);
 #pragma unroll
           for (int k = 0; k < V; ++k) v[k] = s < len ? v[k] : 0.f;
-          if (s < a.T && me.on) store_vec<T, V>((T*)a.y + row_of(a, b, s, len) * a.D + me.c, v);
+          if (s < a.T && me.on) store_vec<T, V>((T*)a.y + time_of(a, s, len) * ystep + ybase, v);
         }
         cx[i] = nx[i];
         cz[i] = nz[i];
@@ -487,6 +492,9 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   const int col = !writer ? TQ * 2 * WN + lane : val < NS ? w * NS + val : WN + w * NS + val - NS;
   const int row = writer ? 2 * WN : 0;
   const int t0 = chunk * a.tpc, t1 = min(t0 + a.tpc, a.Tp / TQ);
+  // outputs of time t: ybase + t ystep; pbc of this block and sequence: t bstep
+  const long ystep = (long)a.B * a.D, ybase = (long)b * a.D + me.c, bstep = (long)a.B * 2 * a.N;
+  float* pbc = a.pbc + ((long)blockIdx.x * a.T * a.B + b) * 2 * a.N;
   float sum_dt = 0.f;
   Group<NS, UR> next;
   next.load(bcw + (long)(ENDS ? t1 * TQ - UR : (t1 - 1) * TQ) * 2 * NS);
@@ -611,17 +619,16 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
       for (int i = 0; i < IT; ++i) {
         const int s = s0 + me.r[i];
         if (me.r[i] < TQ && s < a.T && me.on) {
-          const long at = row_of(a, b, s, len) * a.D + me.c;
+          const long at = time_of(a, s, len) * ystep + ybase;
           store_vec<T, V>((T*)a.dx + at, ox[i]);
           store_vec<T, V>((T*)a.ddelta + at, od[i]);
           if (gate) store_vec<T, V>((T*)a.dz + at, oz[i]);
         }
       }
       for (int i = threadIdx.x; i < TQ * 2 * a.N; i += nt) {
-        const int r = i / (2 * a.N), j = i - r * 2 * a.N, s = s0 + r;
+        const int r = a.by2n.div(i), j = i - r * 2 * a.N, s = s0 + r;
         if (s < a.T)
-          a.pbc[((long)blockIdx.x * a.T * a.B + row_of(a, b, s, len)) * 2 * a.N + j] =
-              sbc[r * 2 * WN + (j < a.N ? j : WN + j - a.N)];
+          pbc[time_of(a, s, len) * bstep + j] = sbc[r * 2 * WN + (j < a.N ? j : WN + j - a.N)];
       }
     }
     __syncthreads();
@@ -828,6 +835,7 @@ KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V_, const void* x, long ldx, 
   a.A = A; a.skip = skip; a.bias = bias; a.len = len; a.h0 = h0; a.hT = hT; a.hs = hs; a.bc = bc;
   a.y = y;
   a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse; a.log_a = log_a;
+  a.by2n = FastDiv(N > 0 ? 2 * N : 1);
   if (ssm::bad(a) || (V_ != 1 && V_ != 4)) return hipErrorInvalidValue;
   const ssm::Plan p = ssm::plan(T, B, D, N);
   a.W = p.W; a.Tp = p.Tp;
@@ -863,6 +871,7 @@ KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V_, const void* dy, long ldy,
   a.A = A; a.skip = skip; a.bias = bias; a.len = len; a.hs = const_cast<float*>(hs); a.bc = bc;
   a.dhT = dhT; a.dh0 = dh0; a.dx = dx; a.ddelta = ddelta; a.dz = dz;
   a.T = T; a.B = B; a.D = D; a.N = N; a.softplus = softplus; a.reverse = reverse; a.log_a = log_a;
+  a.by2n = FastDiv(N > 0 ? 2 * N : 1);
   if (ssm::bad(a) || (V_ != 1 && V_ != 4) || !ws || !hs) return hipErrorInvalidValue;
   const ssm::Plan p = ssm::plan(T, B, D, N);
   a.W = p.W; a.Tp = p.Tp;

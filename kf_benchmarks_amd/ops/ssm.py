@@ -48,24 +48,29 @@ MAX_STATES, MAX_TAPS = 64, 8
 
 # ------------------------------------------------------------------- arguments
 def _rows(t):
-    """(t, elements from one row to the next) of [..., K] read as rows in
+    """(t, elements from one row to the next) of [T, B, K] read as rows in
     order, copied only if its rows are not evenly spaced."""
-    if t.stride(-1) != 1 and t.shape[-1] != 1:
-        t = t.contiguous()
-    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
-    if not lead:
-        return t, t.shape[-1]
-    if len(lead) == 2 and lead[0][1] != lead[1][0] * lead[1][1]:
-        t = t.contiguous()
-        return t, t.shape[-1]
-    return t, lead[-1][1]
+    if t.is_contiguous():
+        return t, t.shape[2]
+    T, B, K = t.shape
+    s0, s1, s2 = t.stride()
+    if (s2 != 1 and K != 1) or (T != 1 and B != 1 and s0 != B * s1):
+        return t.contiguous(), K
+    return t, (s1 if B != 1 else s0 if T != 1 else K)
 
 
 def _vec(width, elems, *rows):
     """Whether every (tensor, row stride) and a width allow ``elems``-wide loads."""
-    return width % elems == 0 and all(
-        t is None or (ld % elems == 0 and t.data_ptr() % (elems * t.element_size()) == 0)
-        for t, ld in rows)
+    if width % elems:
+        return False
+    at = lds = 0
+    size = 1
+    for t, ld in rows:
+        if t is not None:
+            at |= t.data_ptr()
+            lds |= ld
+            size = t.element_size()
+    return lds % elems == 0 and at % (elems * size) == 0  # (powers of two)
 
 
 def _same(x, shape, **tensors):
