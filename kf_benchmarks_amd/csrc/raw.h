@@ -26,6 +26,12 @@ template <typename T, int V> struct Raw {
     }
   }
 
+  // zero unless ``on``
+  __device__ __forceinline__ void keep(bool on) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i) d[i] = on ? d[i] : 0;
+  }
+
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < ND; ++i) d[i] = 0;

@@ -462,3 +462,27 @@ def test_same_bits_and_sinks_gpu(cuda):
     for k, p in ps.items():
         assert p.grad is None
         torch.testing.assert_close(p._kfb_grad_sink, (a if k in a and k != "w" and k != "b" else ca)[k] + 3, rtol=1e-6, atol=1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [2, 4, 6])
+def test_causal_conv_infinite_inputs_gpu(cuda, K):
+    """An infinite input reaches the outputs and gradients of its own channel and window alone."""
+    T, B, D = 37, 2, 24
+    i, dy, _ = conv_inputs(T, B, D, K, torch.float32, cuda, act=None)
+    i["lengths"] = torch.tensor([20, 37], dtype=torch.int32, device=cuda)
+    clean = conv_run(i, dy)
+    x = i["x"].clone()
+    x[19, 0, 3], x[5, 1, 7] = float("inf"), float("nan")
+    i["x"] = x
+    got = conv_run(i, dy)
+    bad = torch.zeros(T, B, D, dtype=torch.bool, device=cuda)
+    bad[19:20, 0, 3] = True
+    bad[5:5 + K, 1, 7] = True
+    assert torch.equal(~torch.isfinite(got["y"]), bad)
+    assert torch.equal(got["x"], clean["x"]) and torch.equal(got["b"], clean["b"])
+    bad = torch.zeros(K, D, dtype=torch.bool, device=cuda)
+    bad[:, 7] = True
+    bad[K - 1, 3] = True  # of sequence 0 only its last row sees the infinity, through the last tap
+    assert torch.equal(~torch.isfinite(got["w"]), bad)
+    assert torch.equal(got["w"][~bad], clean["w"][~bad])
