@@ -755,10 +755,13 @@ struct Plan {
   int fc, bc;  // chunks of the forward and of the backward
 };
 
-// A sequence is cut where its workgroups alone leave the card idle: up to
-// ``want`` workgroups, each at least 4 tiles long.
-inline int chunks_of(long wgs, int tiles, long want) {
-  long c = wgs >= want / 2 ? 1 : want / wgs;
+// A sequence is cut where its workgroups alone leave the card idle (fewer than
+// ``alone``), into ``want`` workgroups of at least 4 tiles.  Forward at 874 steps of
+// 1600 channels, 16 states: 16 sequences (400 workgroups) 255 us whole, 226 in 800
+// workgroups, 183 in 2000; 32 sequences (800) 286 us whole, 341 in 1600.  Backward,
+// two workgroups a compute unit: 16 sequences 535 us whole, 600 in 2000.
+inline int chunks_of(long wgs, int tiles, long alone, long want) {
+  long c = wgs >= alone ? 1 : want / wgs;
   if (c > tiles / 4) c = tiles / 4;
   return (int)(c < 1 ? 1 : c > 65535 ? 65535 : c);
 }
@@ -772,8 +775,8 @@ inline Plan plan(int T, int B, int D, int N) {
   p.tiles = ceil_div(T, p.tq);
   p.Tp = p.tiles * p.tq;
   const long wgs = (long)ceil_div(D, 64) * B;
-  p.fc = chunks_of(wgs, p.tiles, 2048);
-  p.bc = chunks_of(wgs, p.tiles, 512);
+  p.fc = chunks_of(wgs, p.tiles, 640, 2048);
+  p.bc = chunks_of(wgs, p.tiles, 256, 512);
   return p;
 }
 
