@@ -9,7 +9,8 @@
 // with the last K inputs (backward: also the last K gradients of u) in registers
 // and a batch of loads in flight: each input is read once, and the K - 1 rows next to a
 // run once more (from cache).  u is computed again in the backward, nothing but x
-// is kept.
+// is kept.  874 x 16 x 1600 bf16 values, 4 taps, SiLU: 22.3 us forward (4.0 TB/s; a
+// copy reaches 5.2), 45 us backward (3.0 TB/s).
 #include "act.h"
 #include "raw.h"
 

@@ -17,8 +17,10 @@
 // loaded while a tile is walked.
 //
 // Bound by the vector units: an exponential (8 cycles a wave) and four fused
-// operations (4 cycles each) per state, 24 cycles; the bytes take a quarter to
-// a half of that.  Where B D / 64 workgroups do not fill the card, a sequence is
+// operations (4 cycles each) per state, 24 cycles, and about 60 operations a value
+// around it; the bytes take a quarter to a half of that.  With 16 states 874 x 64 x
+// 1600 bf16 values take 460 us, 5.1 ps each, two thirds of the vector units' rate
+// (of the rest, the walks' scalar loads and barriers have most).  Where B D / 64 workgroups do not fill the card, a sequence is
 // cut into chunks: ends_k walks every chunk but the last from a zero state, and
 // because the decays of a chunk multiply to exp(A sum dt), the state before a
 // chunk follows from the earlier chunks' (end, sum dt) alone.
@@ -92,6 +94,7 @@ __device__ __forceinline__ long row_of(const Args& a, int b, int s, int len) {
   return time_of(a, s, len) * a.B + b;
 }
 
+// (5 us for 874 x 16 rows of 16 states.)
 // B and C in fp32, per wave, zero past a sequence's end and past N (a row that
 // must not count may hold NaN).
 template <typename T, int NS>
@@ -399,7 +402,11 @@ template <int M> __device__ __forceinline__ int lane_value(int l) {
 //   dA = sum_t g dt a h_{t-1};  dB = sum_d g dt x;  dC = sum_d e h.
 // dB and dC are summed over the wave's 64 channels here and over the channel
 // blocks by bc_grad_k, dA, dskip and dbias over the chunks by param_grad_k: no
-// atomics, the same sums on every run.
+// atomics, the same sums on every run.  Bound by the vector units too: 70
+// instructions a step of 4 states (19 of them the sums over lanes), 1840 a wave and tile,
+// at two waves a SIMD (H and dec take 128 registers): 874 x 16 x 1600 values take
+// 500 us.  Tiles of 8 steps (three waves a SIMD), decays computed again instead of
+// kept, and two states a wave were no faster (550 to 890 us).
 // ENDS: only the gradient before each chunk, from zero behind it, and sum dt.
 template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
 __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
@@ -717,7 +724,8 @@ param_grad_k(const float* __restrict__ p, int S, int N, int D, const float* log_
 }
 
 // One token: state [B][N][D] in place.  64 channels x 4 waves, wave w the
-// states w, w + 4, ...
+// states w, w + 4, ...  64 x 16 x 1600 states, 13 MB read and written: 5.8 us
+// (2.3 TB/s: short of work for the card's 256 units, and the launch is 3.5).
 template <typename T>
 __global__ void __launch_bounds__(256) step_k(Args a, float* __restrict__ state) {
   __shared__ float yp[4][64];

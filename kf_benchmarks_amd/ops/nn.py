@@ -620,6 +620,18 @@ def size_query(name, *args):
     return N.query(name, *args)
 
 
+def first_order(backward):
+    """A Function's backward that refuses to be differentiated again.  Only a
+    backward that builds a graph (create_graph) pays for the check."""
+    once = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 def on_device(x):
     """Context in which ``x``'s device is the current one (kernels launch on
     the current device, whatever stream they are given)."""
@@ -662,7 +674,7 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @first_order
     def backward(ctx, dy):
         x, gamma, beta, st = ctx.saved_tensors
         groups, act = ctx.args

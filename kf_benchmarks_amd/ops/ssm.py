@@ -24,7 +24,6 @@ oracle of the GPU tests).
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import nn as F_ops
@@ -181,7 +180,7 @@ class _CausalConv(torch.autograd.Function):
         return (y, last) if state else y
 
     @staticmethod
-    @once_differentiable
+    @F_ops.first_order
     def backward(ctx, dy, dlast=None):
         x, w, b, initial, lengths = ctx.saved_tensors
         act, reverse, state = ctx.args
@@ -346,7 +345,7 @@ class _SelectiveScan(torch.autograd.Function):
         return (y, hT) if state else y
 
     @staticmethod
-    @once_differentiable
+    @F_ops.first_order
     def backward(ctx, dy, dhT=None):
         x, delta, A, D, z, bias, lengths, bc, hs = ctx.saved_tensors
         softplus, reverse, log_A, has_h0 = ctx.args
@@ -491,7 +490,7 @@ class _SplitColumns(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
+    @F_ops.first_order
     def backward(ctx, *grads):
         offs = [0]
         for w in ctx.widths:
