@@ -312,10 +312,10 @@ inline bool bad(const Args& a) {
 }
 
 // Positions of a thread's run: long runs read few rows twice, short ones fill the
-// card (2048 waves).
+// card (2048 waves).  A launch has at most 65535 runs.
 inline int run_of(long T, long lanes) {
   int run = 64;
-  while (run > 8 && lanes * ceil_div(T, run) < 2048 * 64) run /= 2;
+  while (run > 8 && lanes * ceil_div(T, run) < 2048 * 64 && ceil_div(T, run / 2) < 65000) run /= 2;
   return run;
 }
 
@@ -348,6 +348,7 @@ using namespace kfb;
 KFB_API int kfb_cconv_max_taps() { return cconv::KMAX; }
 
 KFB_API long kfb_cconv_bwd_ws(int T, int B, int D, int K) {
+  if (T <= 0 || B <= 0 || D <= 0 || K <= 0) return 0;
   return (long)cconv::bwd_slabs(T, B, D, cconv::run_of(T, (long)ceil_div(D, cconv::BV) * B)) * (K + 1) * D;
 }
 

@@ -818,6 +818,7 @@ inline int vec(int dtype, int C, const void* p, const void* q, const void* r) {
 // alignment of the tensors.
 KFB_API long kfb_gn_fwd_ws(int dtype, long N, long HW, int C, int G) {
   long most = 0;
+  if (gn::bad(N, HW, C, G)) return 0;
   for (int v : {1, 2, 4, 8})
     if (C % v == 0) {
       const long w = gn::plan(dtype, N, HW, C, G, v, false).ws;
@@ -828,6 +829,7 @@ KFB_API long kfb_gn_fwd_ws(int dtype, long N, long HW, int C, int G) {
 
 KFB_API long kfb_gn_bwd_ws(int dtype, long N, long HW, int C, int G) {
   long most = 0;
+  if (gn::bad(N, HW, C, G)) return 0;
   for (int v : {1, 2, 4, 8})
     if (C % v == 0) {
       const long w = gn::plan(dtype, N, HW, C, G, v, true).ws;

@@ -823,6 +823,7 @@ KFB_API int kfb_ssm_max_states() { return 64; }
 // Floats of: the fp32 copy of B and C and the forward's chunk ends (what = 0),
 // the saved states of a training forward (1), the backward's workspace (2).
 KFB_API long kfb_ssm_floats(int what, int T, int B, int D, int N) {
+  if (T <= 0 || B <= 0 || D <= 0 || N <= 0) return 0;
   const ssm::Plan p = ssm::plan(T, B, D, N);
   const long state = (long)B * N * D, chunk = state + (long)B * D;
   switch (what) {

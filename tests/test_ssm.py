@@ -486,3 +486,17 @@ def test_causal_conv_infinite_inputs_gpu(cuda, K):
     bad[K - 1, 3] = True  # of sequence 0 only its last row sees the infinity, through the last tap
     assert torch.equal(~torch.isfinite(got["w"]), bad)
     assert torch.equal(got["w"][~bad], clean["w"][~bad])
+
+
+@pytest.mark.gpu
+def test_causal_conv_many_short_runs_gpu(cuda):
+    """2^20 positions of one narrow sequence: as many runs as a launch takes."""
+    x = torch.randn(1 << 20, 1, 8, device=cuda)
+    w = torch.randn(2, 8, device=cuda)
+    y, last = ssm.causal_conv(x, w, return_state=True)
+    want = w[1] * x
+    want[1:] += w[0] * x[:-1]
+    torch.testing.assert_close(y, want, rtol=1e-6, atol=1e-6)
+    assert torch.equal(last, x[-1:])
+    with pytest.raises(ValueError):
+        ssm.causal_conv(torch.zeros((1 << 20) + 1, 1, 1, device=cuda), w[:, :1].contiguous())
