@@ -620,6 +620,27 @@ def size_query(name, *args):
     return N.query(name, *args)
 
 
+def grad_buffers(params):
+    """(gradient tensors for a kernel to write, 1 where that is a parameter's
+    flat-buffer gradient to add to).  A parameter given twice has one of them: the kernel adds to
+    each tensor without knowing of the other."""
+    out, acc = [], []
+    for k, p in enumerate(params):
+        sink = _grad_sink(p) if not any(p is q for q in params[:k]) else None
+        acc.append(int(sink is not None))
+        out.append(sink if sink is not None or p is None else torch.empty_like(p))
+    return out, acc
+
+
+def grads_out(params, grads, acc):
+    """What a backward returns for them: None where it is in the flat buffer."""
+    for k, p in enumerate(params):
+        if acc[k]:
+            _grad_ready(p)
+            grads[k] = None
+    return grads
+
+
 def first_order(backward):
     """A Function's backward that refuses to be differentiated again.  Only a
     backward that builds a graph (create_graph) pays for the check."""
@@ -682,21 +703,14 @@ class _GroupNorm(torch.autograd.Function):
         C, n, dev = x.shape[-1], x.shape[0], x.device
         hw = x.numel() // (n * C)
         dx = torch.empty_like(x)
-        sinks = [_grad_sink(p) for p in ctx.params]
-        grads = [s if s is not None or p is None else torch.empty((C,), dtype=torch.float32,
-                                                                  device=dev)
-                 for s, p in zip(sinks, ctx.params)]
+        grads, acc = grad_buffers(ctx.params)
         ws = x.new_empty((size_query("kfb_gn_bwd_ws", N.dt(x), n, hw, C, groups),),
                          dtype=torch.float32)
         base = st.data_ptr()
         N.call("kfb_gn_bwd", N.dt(x), dy.data_ptr(), x.data_ptr(), dx.data_ptr(), n, hw, C, groups,
                N.ptr(gamma), N.ptr(beta), act, base, base + 4 * n * groups, N.ptr(grads[0]),
-               N.ptr(grads[1]), int(sinks[0] is not None), int(sinks[1] is not None),
-               ws.data_ptr(), N.stream(dev))
-        for k, p in enumerate(ctx.params):
-            if sinks[k] is not None:
-                _grad_ready(p)
-                grads[k] = None
+               N.ptr(grads[1]), acc[0], acc[1], ws.data_ptr(), N.stream(dev))
+        grads = grads_out(ctx.params, grads, acc)
         return dx, grads[0], grads[1], None, None, None
 
 

@@ -108,21 +108,6 @@ def _rows2(t):
     return (t, s0) if s1 == 1 or t.shape[1] == 1 else (t.contiguous(), t.shape[1])
 
 
-def _grad_buffers(params):
-    """(gradient tensors to write, whether each is a flat-buffer sink to add to)"""
-    sinks = [F_ops._grad_sink(p) for p in params]
-    out = [s if s is not None or p is None else torch.empty_like(p) for s, p in zip(sinks, params)]
-    return out, [int(s is not None) for s in sinks]
-
-
-def _grads_out(params, grads, acc):
-    for k, p in enumerate(params):
-        if acc[k]:
-            F_ops._grad_ready(p)
-            grads[k] = None
-    return grads
-
-
 def _positions(x, lengths, reverse):
     """[T, B] row of each position (its own inverse) and [T, B, 1] whether the
     position is inside its sequence."""
@@ -193,14 +178,14 @@ class _CausalConv(torch.autograd.Function):
         dlast = dlast.contiguous() if dlast is not None else None
         dx = torch.empty((T, B, D), dtype=x.dtype, device=dev)
         dinit = torch.empty_like(initial) if initial is not None and ctx.needs_input_grad[3] else None
-        grads, acc = _grad_buffers(ctx.params)
+        grads, acc = F_ops.grad_buffers(ctx.params)
         ws = torch.empty((F_ops.size_query("kfb_cconv_bwd_ws", T, B, D, K),), dtype=torch.float32, device=dev)
         N.call("kfb_cconv_bwd", N.dt(x),
                int(_vec(D, 4, (x, ldx), (dy, ldy), (initial, D), (dlast, D))), dy.data_ptr(), ldy,
                x.data_ptr(), ldx, N.ptr(initial), w.data_ptr(), N.ptr(b), N.ptr(lengths),
                N.ptr(dlast), dx.data_ptr(), N.ptr(dinit), N.ptr(grads[0]), N.ptr(grads[1]), acc[0],
                acc[1], ws.data_ptr(), T, B, D, K, act, int(reverse), N.stream(dev))
-        grads = _grads_out(ctx.params, grads, acc)
+        grads = F_ops.grads_out(ctx.params, grads, acc)
         return dx, grads[0], grads[1], dinit, None, None, None, None
 
 
@@ -247,8 +232,8 @@ def causal_conv(x, w, b=None, activation=None, lengths=None, initial_state=None,
 
 
 def causal_conv_step(x, state, w, b=None, activation=None):
-    """One token x [B, D] after ``state`` [K-1, B, D] (x's type, contiguous), which
-    is moved on in place: y [B, D].  No gradient."""
+    """One token x [B, D] after ``state`` [K-1, B, D] (x's type, contiguous, sharing
+    no memory with x), which is moved on in place: y [B, D].  No gradient."""
     act = F_ops.fused_act_code(activation)
     if x.dim() != 2 or x.numel() == 0:
         raise ValueError("causal_conv_step: a non-empty [B, D] tensor expected, got %s" %
@@ -361,7 +346,7 @@ class _SelectiveScan(torch.autograd.Function):
         dx, ddelta = (torch.empty((T, Bn, Dn), dtype=dt, device=dev) for _ in range(2))
         dz = torch.empty((T, Bn, Dn), dtype=dt, device=dev) if z is not None else None
         dB, dC = (torch.empty((T, Bn, Ns), dtype=dt, device=dev) for _ in range(2))
-        grads, acc = _grad_buffers(ctx.params)
+        grads, acc = F_ops.grad_buffers(ctx.params)
         ws = torch.empty((F_ops.size_query("kfb_ssm_floats", 2, T, Bn, Dn, Ns),), **f32)
         V = 4 if _vec(Dn, 4, (x, ldx), (delta, ldd), (z, ldz), (dy, ldy)) else 1
         N.call("kfb_ssm_scan_bwd", N.dt(x), V, dy.data_ptr(), ldy, x.data_ptr(), ldx,
@@ -370,7 +355,7 @@ class _SelectiveScan(torch.autograd.Function):
                ddelta.data_ptr(), N.ptr(dz), dB.data_ptr(), dC.data_ptr(), N.ptr(grads[0]),
                N.ptr(grads[1]), N.ptr(grads[2]), acc[0], acc[1], acc[2], ws.data_ptr(), T, Bn, Dn,
                Ns, int(softplus), int(reverse), int(log_A), N.stream(dev))
-        dA, dD, dbias = _grads_out(ctx.params, grads, acc)
+        dA, dD, dbias = F_ops.grads_out(ctx.params, grads, acc)
         return dx, ddelta, dA, dB, dC, dD, dz, dbias, dh0, None, None, None, None, None
 
 
@@ -508,6 +493,8 @@ def split_columns(x, widths):
     if sum(widths) != x.shape[-1]:
         raise ValueError("split_columns: %d columns do not split into %s" % (x.shape[-1],
                                                                            tuple(widths)))
+    if len(widths) > F_ops._CAT_MAX:
+        raise ValueError("split_columns: at most %d slices" % F_ops._CAT_MAX)
     if not x.is_cuda or not x.requires_grad:
         return torch.split(x, list(widths), dim=-1)
     return _SplitColumns.apply(x.contiguous(), tuple(widths))

@@ -500,3 +500,22 @@ def test_causal_conv_many_short_runs_gpu(cuda):
     assert torch.equal(last, x[-1:])
     with pytest.raises(ValueError):
         ssm.causal_conv(torch.zeros((1 << 20) + 1, 1, 1, device=cuda), w[:, :1].contiguous())
+
+
+@pytest.mark.gpu
+def test_one_parameter_twice_gpu(cuda):
+    """One tensor given as skip and as bias: its flat-buffer gradient is the sum of both."""
+    i, dy, _ = scan_inputs(40, 2, 72, 5, torch.float32, cuda)
+    p = i["D"].clone().requires_grad_()
+    want = torch.autograd.grad(ssm.selective_scan(i["x"], i["delta"], i["A"], i["B"], i["C"], p, i["z"], p), p, dy)[0]
+    q = i["D"].clone().requires_grad_()
+    q._kfb_grad_sink = torch.zeros_like(q)
+    y = ssm.selective_scan(i["x"], i["delta"], i["A"], i["B"], i["C"], q, i["z"], q)
+    y.backward(dy)
+    torch.testing.assert_close(q._kfb_grad_sink + q.grad, want, rtol=1e-6, atol=1e-6)
+
+
+def test_split_columns_too_many_slices():
+    n = ssm.F_ops._CAT_MAX + 1
+    with pytest.raises(ValueError, match="at most"):
+        ssm.split_columns(torch.zeros(2, n), (1,) * n)
