@@ -622,8 +622,8 @@ def size_query(name, *args):
 
 def grad_buffers(params):
     """(gradient tensors for a kernel to write, 1 where that is a parameter's
-    flat-buffer gradient to add to).  A parameter given twice has one of them: the kernel adds to
-    each tensor without knowing of the other."""
+    flat-buffer gradient to add to).  A parameter given twice has one of them: the
+    kernel adds to each tensor without knowing of the other."""
     out, acc = [], []
     for k, p in enumerate(params):
         sink = _grad_sink(p) if not any(p is q for q in params[:k]) else None

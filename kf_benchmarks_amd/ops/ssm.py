@@ -239,7 +239,7 @@ def causal_conv_step(x, state, w, b=None, activation=None):
         raise ValueError("causal_conv_step: a non-empty [B, D] tensor expected, got %s" %
                          (tuple(x.shape),))
     B, D = x.shape
-    K, dt, dev = w.shape[0], x.dtype, x.device
+    K, dt, dev = w.shape[0] if w.dim() else 0, x.dtype, x.device
     # (one token: the checks are a good part of the call, so the messages are left
     # to the slow ones)
     if not (1 <= K <= MAX_TAPS and F_ops.fits_param(w, (K, D), dev) and F_ops.fits_param(b, (D,), dev)
@@ -386,15 +386,15 @@ def selective_scan(x, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
 
     A, D [D], delta_bias [D] fp32; D, z, delta_bias may be None.  dt A is meant to be
     finite and not positive; ``log_A``: A is given as log(-A), the form that training
-    keeps negative (its gradient is that of the logarithm).  ``initial_state``: h before the first row (zero if
-    None); ``return_state``: also h after each sequence's last row, from which
-    selective_scan or selective_scan_step goes on.  Differentiable once in every
-    tensor but ``lengths``."""
+    keeps negative (its gradient is that of the logarithm).  ``initial_state``: h
+    before the first row (zero if None); ``return_state``: also h after each
+    sequence's last row, from which selective_scan or selective_scan_step goes on.
+    Differentiable once in every tensor but ``lengths``."""
     if x.dim() != 3 or x.numel() == 0:
         raise ValueError("selective_scan: a non-empty [T, B, D] tensor expected, got %s" %
                          (tuple(x.shape),))
     T, Bn, Dn = shape = x.shape
-    dt, dev, Ns = x.dtype, x.device, A.shape[0]
+    dt, dev, Ns = x.dtype, x.device, A.shape[0] if A.dim() else 0
     if not (1 <= Ns <= MAX_STATES and _fits(delta, shape, dt, dev) and _fits(z, shape, dt, dev)
             and _fits(B, (T, Bn, Ns), dt, dev) and _fits(C, (T, Bn, Ns), dt, dev)
             and F_ops.fits_param(A, (Ns, Dn), dev) and F_ops.fits_param(D, (Dn,), dev)
@@ -428,7 +428,7 @@ def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=Non
                          (tuple(x.shape),))
     shape, dt, dev = x.shape, x.dtype, x.device
     Bn, Dn = shape
-    Ns = A.shape[0]
+    Ns = A.shape[0] if A.dim() else 0
     if not (1 <= Ns <= MAX_STATES and Bn <= 65535 and _fits(delta, shape, dt, dev)
             and _fits(z, shape, dt, dev) and _fits(B, (Bn, Ns), dt, dev)
             and _fits(C, (Bn, Ns), dt, dev) and F_ops.fits_param(A, (Ns, Dn), dev)

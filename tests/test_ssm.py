@@ -519,3 +519,15 @@ def test_split_columns_too_many_slices():
     n = ssm.F_ops._CAT_MAX + 1
     with pytest.raises(ValueError, match="at most"):
         ssm.split_columns(torch.zeros(2, n), (1,) * n)
+
+
+def test_scalar_parameters_are_refused():
+    x, s = torch.zeros(2, 3, 4), torch.zeros(())
+    with pytest.raises(ValueError):
+        ssm.selective_scan(x, x, s, x[..., :1], x[..., :1])
+    with pytest.raises(ValueError):
+        ssm.selective_scan_step(x[0], x[0], s, x[0, :, :1], x[0, :, :1], torch.zeros(3, 1, 4))
+    with pytest.raises(ValueError):
+        ssm.causal_conv(x, s)
+    with pytest.raises(ValueError):
+        ssm.causal_conv_step(x[0], x[:1].contiguous(), s)
