@@ -236,14 +236,21 @@ KFB_API hipError_t kfb_seqlock_check(const long long* seq, long long expect, int
 }
 
 // Page-locks host memory (e.g. a /dev/shm mapping) for device access;
-// *dev receives its device address.
+// *dev receives its device address.  Some systems refuse this, and callers go on
+// without it: the error is returned and not left behind, where the thread's next
+// launch, of whoever it is, would report it as its own.
 KFB_API hipError_t kfb_host_register(void* p, size_t bytes, void** dev) {
   hipError_t e = hipHostRegister(p, bytes, hipHostRegisterMapped);
-  if (e != hipSuccess) return e;
-  return hipHostGetDevicePointer(dev, p, 0);
+  if (e == hipSuccess && (e = hipHostGetDevicePointer(dev, p, 0)) != hipSuccess) (void)hipHostUnregister(p);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
 }
 
-KFB_API hipError_t kfb_host_unregister(void* p) { return hipHostUnregister(p); }
+KFB_API hipError_t kfb_host_unregister(void* p) {
+  const hipError_t e = hipHostUnregister(p);
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e;
+}
 
 // ---------------------------------------------------------------------------
 // Peer model slots over HIP IPC (KungFu PairAveraging, parallel/kungfu.py).

@@ -336,3 +336,17 @@ def test_bench_selftest_fallback_rebuilds_hierarchical(cuda):
     assert any(f.startswith("hier:") for f in st["failed"]), st["failed"]
     assert out["backend"] == "nccl" and out["comm"]["native_comms_live"] == 0
     assert out["weights_in_sync"] is True and out["value"] > 0
+
+
+def test_refused_host_registration_leaves_no_error(cuda):
+    """A refused page-lock raises where it is asked for; the next launch, which
+    has nothing to do with it, runs."""
+    import ctypes
+    import torch
+    from kf_benchmarks_amd.ops import _native as N
+    x = torch.zeros(8, device=cuda)
+    dev = ctypes.c_void_p()
+    with pytest.raises(N.NativeError):
+        N.call("kfb_host_register", None, 0, ctypes.byref(dev))
+    x.fill_(3.0)
+    assert float(x.sum()) == 24.0
