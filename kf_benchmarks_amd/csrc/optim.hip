@@ -23,6 +23,8 @@
 #include "common.h"
 
 #include <cstring>
+#include <mutex>
+#include <vector>
 
 namespace kfb {
 
@@ -229,25 +231,97 @@ KFB_API hipError_t kfb_cast_f32(const float* x, void* y, int dtype, long n, hipS
   return hipGetLastError();
 }
 
+// Host memory (a /dev/shm mapping) whose words kfb_seqlock_check reads.  It is
+// page-locked for the device where the system allows that for memory that exists
+// already.  Where it is refused, the words get a page-locked copy of their own, and
+// each check first brings its word up to date by a host call in stream order: after
+// what was enqueued before it (the copy of the model), as the kernel's own read is.
+namespace kfb {
+
+struct Staged {
+  char* host;
+  char* pinned;  // of the host's address as of the device's
+  char* dev;
+  size_t bytes;
+};
+static std::mutex staged_mu;
+static std::vector<Staged> staged;
+
+struct WordCopy {
+  const long long* from;
+  long long* to;
+};
+
+static void copy_word(void* p) {
+  WordCopy* w = (WordCopy*)p;
+  __atomic_store_n(w->to, __atomic_load_n(w->from, __ATOMIC_ACQUIRE), __ATOMIC_RELEASE);
+  delete w;
+}
+
+}  // namespace kfb
+
 KFB_API hipError_t kfb_seqlock_check(const long long* seq, long long expect, int* ok, int* torn,
                                      hipStream_t stream) {
+  WordCopy* w = nullptr;
+  {
+    std::lock_guard<std::mutex> lock(staged_mu);
+    for (const Staged& m : staged) {
+      const size_t at = (size_t)((const char*)seq - m.dev);
+      if ((const char*)seq >= m.dev && at + sizeof(long long) <= m.bytes)
+        w = new WordCopy{(const long long*)(m.host + at), (long long*)(m.pinned + at)};
+    }
+  }
+  if (w) {
+    const hipError_t e = hipLaunchHostFunc(stream, copy_word, w);
+    if (e != hipSuccess) {
+      delete w;
+      return e;
+    }
+  }
   hipLaunchKernelGGL(seqlock_check_k, dim3(1), dim3(1), 0, stream, seq, expect, ok, torn);
   return hipGetLastError();
 }
 
-// Page-locks host memory (e.g. a /dev/shm mapping) for device access;
-// *dev receives its device address.  Some systems refuse this, and callers go on
-// without it: the error is returned and not left behind, where the thread's next
+// Makes host memory p readable by kfb_seqlock_check; *dev receives the address to
+// give it.  An error is returned and not left behind, where the thread's next
 // launch, of whoever it is, would report it as its own.
 KFB_API hipError_t kfb_host_register(void* p, size_t bytes, void** dev) {
+  if (!p || !bytes || !dev) return hipErrorInvalidValue;
   hipError_t e = hipHostRegister(p, bytes, hipHostRegisterMapped);
-  if (e == hipSuccess && (e = hipHostGetDevicePointer(dev, p, 0)) != hipSuccess) (void)hipHostUnregister(p);
-  if (e != hipSuccess) (void)hipGetLastError();
-  return e;
+  if (e == hipSuccess) {
+    if ((e = hipHostGetDevicePointer(dev, p, 0)) == hipSuccess) return e;
+    (void)hipHostUnregister(p);
+  }
+  (void)hipGetLastError();
+  Staged m{(char*)p, nullptr, nullptr, bytes};
+  e = hipHostMalloc((void**)&m.pinned, bytes, hipHostMallocMapped);
+  if (e == hipSuccess && (e = hipHostGetDevicePointer((void**)&m.dev, m.pinned, 0)) != hipSuccess)
+    (void)hipHostFree(m.pinned);
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    return e;
+  }
+  memcpy(m.pinned, p, bytes);
+  std::lock_guard<std::mutex> lock(staged_mu);
+  staged.push_back(m);
+  *dev = m.dev;
+  return hipSuccess;
 }
 
+// (waits for checks under way, which still read p)
 KFB_API hipError_t kfb_host_unregister(void* p) {
-  const hipError_t e = hipHostUnregister(p);
+  hipError_t e = hipDeviceSynchronize();
+  if (e != hipSuccess) return e;
+  {
+    std::lock_guard<std::mutex> lock(staged_mu);
+    for (size_t i = 0; i < staged.size(); ++i)
+      if (staged[i].host == (char*)p) {
+        char* pinned = staged[i].pinned;
+        staged.erase(staged.begin() + i);
+        return hipHostFree(pinned);
+      }
+  }
+  e = hipHostUnregister(p);
   if (e != hipSuccess) (void)hipGetLastError();
   return e;
 }

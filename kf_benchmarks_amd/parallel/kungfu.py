@@ -92,8 +92,9 @@ class _Header:
         struct.pack_into("<q", self._map(self.rank), 8 * word, v)
 
     def device_word(self, r, word):
-        """Device address of peer ``r``'s header word (page-locked host
-        memory); None if the mapping cannot be registered."""
+        """Device address of peer ``r``'s header word for the native seqlock
+        check (page-locked, or a page-locked copy that the check refreshes);
+        None if there is neither."""
         if r not in self._dev:
             import ctypes
             from ..ops import _native as N
