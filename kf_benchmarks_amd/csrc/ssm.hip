@@ -54,6 +54,19 @@ struct Args {
   FastDiv by2n;
 };
 
+// The state from which wave w reads the saved states: its first one.  There are at least
+// four waves, so some may have no state; these loads have no branch, so such a wave reads
+// the last state, and what it reads is dropped.
+__host__ __device__ inline int base_state(int w, int NS, int N) { return w * NS < N ? w * NS : N - 1; }
+
+// Where state n of sequence b, channel d stands in [B][N][D].
+__host__ __device__ inline long state_at(int b, int n, int N, int D, int d) {
+  return ((long)b * N + n) * D + d;
+}
+
+// From a wave's base to its state i, of ns; for a state that it does not have, to the base.
+__host__ __device__ inline long saved_at(int i, int ns, int D) { return i < ns ? (long)i * D : 0; }
+
 // B and C as constant memory: uniform addresses become scalar loads
 typedef const __attribute__((address_space(4))) float cfloat;
 
@@ -215,7 +228,7 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   const int len = seq_len(a, b), ns = min(max(a.N - w * NS, 0), NS);  // states of this wave
   const bool ok = d < a.D;
   const int dc = ok ? d : a.D - 1;
-  const long bnd = ((long)b * a.N + w * NS) * a.D + dc, bn = (long)a.B * a.N * a.D;
+  const long bnd = state_at(b, w * NS, a.N, a.D, dc), bn = (long)a.B * a.N * a.D;
   float A2[NS], h[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
@@ -423,7 +436,8 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   const int len = seq_len(a, b), nt = a.W * 64, ns = min(max(a.N - w * NS, 0), NS);
   const bool ok = d < a.D;
   const int dc = ok ? d : a.D - 1;
-  const long bnd = ((long)b * a.N + w * NS) * a.D + dc, bn = (long)a.B * a.N * a.D;
+  const long bnd = state_at(b, w * NS, a.N, a.D, dc), bn = (long)a.B * a.N * a.D;
+  const long saved = state_at(b, base_state(w, NS, a.N), a.N, a.D, dc);
   float A1[NS], carry[NS], dA[NS];
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
@@ -455,9 +469,9 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
     ly.load(me.r, s0, ny);
     lz.load(me.r, s0, nz);
     if (!ENDS) {
-      const float* hs = a.hs + (long)(s0 / TQ) * bn + bnd;
+      const float* hs = a.hs + (long)(s0 / TQ) * bn + saved;
 #pragma unroll
-      for (int i = 0; i < NS; ++i) hn[i] = hs[i < ns ? (long)i * a.D : 0];
+      for (int i = 0; i < NS; ++i) hn[i] = hs[saved_at(i, ns, a.D)];
     }
   };
   auto stage = [&](int s0) {
@@ -833,6 +847,22 @@ KFB_API long kfb_ssm_floats(int what, int T, int B, int D, int N) {
                    (p.bc > 1 ? p.bc * chunk : 0);
     default: return -1;
   }
+}
+
+// The furthest element of the saved states that the backward reads: every wave's in
+// the last tile of the last sequence and channel.
+KFB_API long kfb_ssm_furthest_state(int T, int B, int D, int N) {
+  if (T <= 0 || B <= 0 || D <= 0 || N <= 0 || N > 64) return -1;
+  const ssm::Plan p = ssm::plan(T, B, D, N);
+  long most = -1;
+  for (int w = 0; w < p.W; ++w)
+    for (int i = 0; i < p.ns; ++i) {
+      const int own = N - w * p.ns, ns = own < 0 ? 0 : own < p.ns ? own : p.ns;
+      const long at = (long)(p.tiles - 1) * B * N * D + ssm::state_at(B - 1, ssm::base_state(w, p.ns, N), N, D, D - 1) +
+                      ssm::saved_at(i, ns, D);
+      if (at > most) most = at;
+    }
+  return most;
 }
 
 KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V_, const void* x, long ldx, const void* delta,

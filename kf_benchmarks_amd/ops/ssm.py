@@ -31,6 +31,7 @@ from . import nn as F_ops
 _I, _L, _P = N.I, N.L, N.P
 N.register_optional("kfb_ssm_max_states", [])
 N.register_optional("kfb_ssm_floats", [_I] * 5, _L)
+N.register_optional("kfb_ssm_furthest_state", [_I] * 4, _L)
 N.register_optional("kfb_ssm_scan_fwd", [_I, _I] + [_P, _L] * 5 + [_P] * 9 + [_I] * 7 + [_P])
 N.register_optional("kfb_ssm_scan_bwd", [_I, _I] + [_P, _L] * 4 + [_P] * 16 + [_I] * 3 + [_P] +
                     [_I] * 7 + [_P])

@@ -531,3 +531,19 @@ def test_scalar_parameters_are_refused():
         ssm.causal_conv(x, s)
     with pytest.raises(ValueError):
         ssm.causal_conv_step(x[0], x[:1].contiguous(), s)
+
+
+@pytest.mark.parametrize("T,B,D", [(1, 1, 1), (16, 1, 64), (40, 3, 130), (1024, 64, 2048), (874, 16, 1600)])
+def test_scan_reads_inside_its_saved_states(T, B, D):
+    """Every wave of the backward, also one without states, reads inside the saved states (the numbers are the
+    kernel's own, evaluated on the host)."""
+    for n in range(1, ssm.MAX_STATES + 1):
+        size, at = N.query("kfb_ssm_floats", 1, T, B, D, n), N.query("kfb_ssm_furthest_state", T, B, D, n)
+        assert size // 2 <= at < size, (n, at, size)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 3, 7, 9, 10, 11, 12, 36])
+def test_selective_scan_partly_filled_waves_gpu(cuda, n):
+    scan_compare(35, 3, 72, n, torch.bfloat16, cuda)
+    scan_compare(70, 2, 33, n, torch.float32, cuda, ragged=True, poison=True, state=True, reverse=True)
