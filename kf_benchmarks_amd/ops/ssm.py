@@ -24,6 +24,7 @@ oracle of the GPU tests).
 from __future__ import annotations
 
 import torch
+from torch.autograd.graph import increment_version  # (a kernel's change of a tensor is torch's to know)
 
 from . import _native as N
 from . import nn as F_ops
@@ -264,6 +265,7 @@ def causal_conv_step(x, state, w, b=None, activation=None):
     with F_ops.on_device(x):
         N.call("kfb_cconv_step", N.dt(x), int(D % ve == 0 and ld % ve == 0 and (px | ps) % 16 == 0),
                px, ld, ps, w.data_ptr(), N.ptr(b), y.data_ptr(), B, D, K, act, N.stream(dev))
+    increment_version(state)
     return y
 
 
@@ -457,6 +459,7 @@ def selective_scan_step(x, delta, A, B, C, state, D=None, z=None, delta_bias=Non
         N.call("kfb_ssm_step", N.dt(x), x.data_ptr(), ldx, delta.data_ptr(), ldd, N.ptr(z), ldz,
                B.data_ptr(), ldb, C.data_ptr(), ldc, A.data_ptr(), N.ptr(D), N.ptr(delta_bias),
                state.data_ptr(), y.data_ptr(), Bn, Dn, Ns, int(softplus), int(log_A), N.stream(dev))
+    increment_version(state)
     return y
 
 

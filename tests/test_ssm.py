@@ -547,3 +547,37 @@ def test_scan_reads_inside_its_saved_states(T, B, D):
 def test_selective_scan_partly_filled_waves_gpu(cuda, n):
     scan_compare(35, 3, 72, n, torch.bfloat16, cuda)
     scan_compare(70, 2, 33, n, torch.float32, cuda, ragged=True, poison=True, state=True, reverse=True)
+
+
+def _steps_count_as_changes(dev):
+    """A step is an in-place change of its state that autograd knows of."""
+    i, _, _ = scan_inputs(3, 2, 8, 4, torch.float32, dev)
+    c, _, _ = conv_inputs(3, 2, 8, 4, torch.float32, dev, state=True)
+    h, s = torch.zeros(2, 4, 8, device=dev), c["state"]
+    w = c["w"].clone().requires_grad_()
+    y = ssm.causal_conv(c["x"], w, c["b"], "silu", initial_state=s)
+    versions = s._version, h._version
+
+    def steps():
+        ssm.causal_conv_step(c["x"][0], s, c["w"], c["b"], "silu")
+        ssm.selective_scan_step(i["x"][0], i["delta"][0], i["A"], i["B"][0], i["C"][0], h)
+
+    with torch.no_grad():
+        steps()
+    assert s._version > versions[0] and h._version > versions[1]
+    with torch.inference_mode():  # tensors made here count no changes
+        h, s = torch.zeros(2, 4, 8, device=dev), torch.zeros(3, 2, 8, device=dev)
+        steps()
+        assert torch.equal(s[-1], c["x"][0]) and h.abs().sum() > 0
+    return y
+
+
+def test_steps_count_as_changes_of_their_state_cpu():
+    _steps_count_as_changes("cpu")
+
+
+@pytest.mark.gpu
+def test_steps_count_as_changes_of_their_state_gpu(cuda):
+    y = _steps_count_as_changes(cuda)
+    with pytest.raises(RuntimeError, match="inplace"):  # the state was kept for the filter's gradient
+        y.sum().backward()
