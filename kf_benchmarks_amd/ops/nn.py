@@ -22,6 +22,7 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _native as N
 from . import conv as _conv
@@ -653,6 +654,13 @@ def first_order(backward):
     return run
 
 
+def has_tangent(*tensors):
+    """Whether one of them carries a forward-mode tangent.  A kernel would drop it: such
+    a call goes through the op's Function, which refuses it."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def on_device(x):
     """Context in which ``x``'s device is the current one (kernels launch on
     the current device, whatever stream they are given)."""
@@ -745,6 +753,7 @@ def group_norm(x, gamma: Optional[torch.Tensor], beta: Optional[torch.Tensor], g
     grad = torch.is_grad_enabled() and (x.requires_grad or
                                         (gamma is not None and gamma.requires_grad) or
                                         (beta is not None and beta.requires_grad))
+    grad = grad or has_tangent(x, gamma, beta)
     with on_device(x):
         if grad:
             return _GroupNorm.apply(x, gamma, beta, int(groups), float(eps), act)

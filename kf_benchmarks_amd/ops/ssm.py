@@ -97,7 +97,7 @@ def _needs_grad(*tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return F_ops.has_tangent(*tensors)
 
 
 def _fits(t, shape, dtype, dev):

@@ -398,3 +398,26 @@ def test_gradient_of_the_state_alone_gpu(cuda):
         _, h = ssm.selective_scan(sx, f(x["delta"]), f(c["A"]), f(x["B"]), f(x["C"]), return_state=True)
         grads.append(torch.autograd.grad(s.sum() + h.sum(), sx)[0])
     assert relerr(grads[1], grads[0]) < 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_tangents_are_refused_gpu(cuda, grad):
+    """No operator drops a tangent: where it has no forward-mode derivative it says so."""
+    import torch.autograd.forward_ad as fw
+    f = lambda *s: torch.ones(s, device=cuda)  # noqa: E731
+    x, delta, A, B, C = f(3, 2, 8), f(3, 2, 8), -f(4, 8), f(3, 2, 4), f(3, 2, 4)
+    w, p, st, h, one = f(2, 8), f(8), f(1, 2, 8), f(2, 4, 8), f(3, 2, 8)
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        d, dp, d0 = fw.make_dual(x, one), fw.make_dual(p, p), fw.make_dual(x[0], one[0])
+        for call in (lambda: F.group_norm(d, None, None, 2), lambda: F.group_norm(x, dp, None, 2),
+                     lambda: ssm.causal_conv(d, w), lambda: ssm.causal_conv(x, w, dp),
+                     lambda: ssm.selective_scan(d, delta, A, B, C),
+                     lambda: ssm.selective_scan(x, delta, A, B, C, delta_bias=dp)):
+            with pytest.raises(NotImplementedError):
+                call()
+        for call in (lambda: ssm.causal_conv_step(d0, st, w),
+                     lambda: ssm.selective_scan_step(d0, delta[0], A, B[0], C[0], h)):
+            with pytest.raises(ValueError):
+                call()
+        F.group_norm(x, None, None, 2)
