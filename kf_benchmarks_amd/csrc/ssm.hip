@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
         if (r < TQ) {
           float v[V];
 #pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = skip[k] * cx[i][k];
+          for (int k = 0; k < V; ++k) v[k] = a.skip ? skip[k] * cx[i][k] : 0.f;  // (not 0 * inf)
           const float* part = yp + r * 64 + me.cl;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {  // W >= 4
@@ -624,9 +624,9 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
         for (int k = 0; k < V; ++k) {
           const float x = in ? cx[i][k] : 0.f, e = me_e.v[k];
           const float sg = sigmoidf(cd[i][k] + bias[k]), dd = fmaf(x, p[k], q[k]);
-          ox[i][k] = in ? fmaf(me_d.v[k], p[k], skip[k] * e) : 0.f;
+          ox[i][k] = in ? fmaf(me_d.v[k], p[k], a.skip ? skip[k] * e : 0.f) : 0.f;
           od[i][k] = in ? (a.softplus ? dd * sg : dd) : 0.f;
-          v[k] = fmaf(skip[k], x, v[k]);
+          v[k] = a.skip ? fmaf(skip[k], x, v[k]) : v[k];
           gskip[k] = fmaf(e, x, gskip[k]);
           gbias[k] += od[i][k];
         }

@@ -581,3 +581,45 @@ def test_steps_count_as_changes_of_their_state_gpu(cuda):
     y = _steps_count_as_changes(cuda)
     with pytest.raises(RuntimeError, match="inplace"):  # the state was kept for the filter's gradient
         y.sum().backward()
+
+
+INF = float("inf")
+
+
+def _mask(shape, dev, *at):
+    m = torch.zeros(shape, dtype=torch.bool, device=dev)
+    for a in at:
+        m[a] = True
+    return m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{}, {"skip": False, "z": False}, {"skip": False}])
+@pytest.mark.parametrize("n", [4, 8, 16, 40])
+def test_selective_scan_infinite_input_gpu(cuda, n, kw):
+    """An infinite input gives infinities, not NaN, and only in what it reaches (with maps and skip of one sign, so that
+    no infinities of opposite signs meet)."""
+    T, B, D, t = 37, 2, 72, 20
+    i, dy, dh = scan_inputs(T, B, D, n, torch.float32, cuda, state=True, **kw)
+    for k in ("B", "C", "D"):
+        i[k] = i[k].abs() if i[k] is not None else None
+    clean = scan_run(i, dy, dh)
+    i["x"] = i["x"].clone()
+    i["x"][t, 0, 3] = INF
+    got = scan_run(i, dy, dh)
+    after, there, row = (slice(t, None), 0, 3), (t, 0, 3), (t, 0)
+    bad = {"y": _mask((T, B, D), cuda, after), "x": _mask((T, B, D), cuda), "delta": _mask((T, B, D), cuda, after),
+           "z": _mask((T, B, D), cuda, after), "A": _mask((n, D), cuda, (slice(None), 3)),
+           "B": _mask((T, B, n), cuda, row), "C": _mask((T, B, n), cuda, (slice(t, None), 0)),
+           "D": _mask((D,), cuda, 3), "bias": _mask((D,), cuda, 3), "state": _mask((B, n, D), cuda),
+           "state_out": _mask((B, n, D), cuda, (0, slice(None), 3))}
+    for k, v in got.items():
+        assert torch.equal(~torch.isfinite(v), bad[k]), k
+        assert torch.equal(v[~bad[k]], clean[k][~bad[k]]), k
+    gate = 1.0 if i["z"] is None else i["z"][after]
+    assert torch.equal(got["y"][after], torch.full((T - t,), INF, device=cuda) * gate)
+    if i["z"] is not None:
+        z = i["z"][after].double()
+        s = torch.sigmoid(z)
+        assert torch.equal(got["z"][after].double(), INF * dy[after].double() * (s * (1 + z * (1 - s))))
+    assert (got["state_out"][0, :, 3] == INF).all()
