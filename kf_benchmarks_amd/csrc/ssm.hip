@@ -217,7 +217,9 @@ __device__ __forceinline__ void join(const Args& a, int b, int dc, long bnd, lon
 // turn: the next tile's rows are fetched before the walk and used before y is stored,
 // so that no wait for a load waits for a store just issued.
 // ENDS: only the state after each chunk, from zero, and the chunk's sum of dt.
-template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
+// PART: not every wave has NS states; those that it does not have stay zero by selection
+// (zero times an infinite input is not).  (ENDS stores none of them.)
+template <typename T, int V, int IT, int NS, int TQ, bool ENDS, bool PART>
 __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   constexpr int UR = 16 / NS < 4 ? 16 / NS : 4;  // steps of a group
@@ -300,7 +302,8 @@ __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
         float v = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          h[i] = fmaf(__builtin_amdgcn_exp2f(u.x * A2[i]), h[i], u.y * bc.B(k, i));
+          const float in = u.y * bc.B(k, i);
+          h[i] = fmaf(__builtin_amdgcn_exp2f(u.x * A2[i]), h[i], PART && i >= ns ? 0.f : in);
           if (!ENDS) v = fmaf(bc.C(k, i), h[i], v);
         }
         if constexpr (ENDS) sum_dt += u.x;
@@ -421,7 +424,8 @@ template <int M> __device__ __forceinline__ int lane_value(int l) {
 // 500 us.  Tiles of 8 steps (three waves a SIMD), decays computed again instead of
 // kept, and two states a wave were no faster (550 to 890 us).
 // ENDS: only the gradient before each chunk, from zero behind it, and sum dt.
-template <typename T, int V, int IT, int NS, int TQ, bool ENDS>
+// PART: as in scan_fwd_k.
+template <typename T, int V, int IT, int NS, int TQ, bool ENDS, bool PART>
 __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int WN = a.W * NS;
@@ -558,7 +562,8 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
             dec[r][i] = __builtin_amdgcn_exp2f(u.x * (A1[i] * LOG2E));
-            H[r][i] = fmaf(dec[r][i], r ? H[r - 1][i] : hb[i], u.y * bc.B(k, i));
+            const float in = u.y * bc.B(k, i);
+            H[r][i] = fmaf(dec[r][i], r ? H[r - 1][i] : hb[i], PART && i >= ns ? 0.f : in);
             v = fmaf(bc.C(k, i), H[r][i], v);
           }
           yp[(w * TQ + r) * 64 + lane] = v;
@@ -891,10 +896,13 @@ KFB_API hipError_t kfb_ssm_scan_fwd(int dtype, int V_, const void* x, long ldx, 
     const size_t shm = (size_t)(2 + p.W) * TQ * 64 * sizeof(float);
     dim3 grid(ceil_div(D, 64), B, a.nchunk - 1);
     if (grid.z)
-      hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, true>), grid, dim3(p.W * 64),
+      hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, true, false>), grid, dim3(p.W * 64),
                          2 * TQ * 64 * sizeof(float), stream, a);
     grid.z = a.nchunk;
-    hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, false>), grid, dim3(p.W * 64), shm, stream, a);
+    if (N == p.W * NS)
+      hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, false, false>), grid, dim3(p.W * 64), shm, stream, a);
+    else
+      hipLaunchKernelGGL((ssm::scan_fwd_k<E, V, IT, NS, TQ, false, true>), grid, dim3(p.W * 64), shm, stream, a);
   }));
   return hipGetLastError();
 }
@@ -931,10 +939,13 @@ KFB_API hipError_t kfb_ssm_scan_bwd(int dtype, int V_, const void* dy, long ldy,
       if (shm < last) shm = last;
       dim3 grid(nblk, B, a.nchunk - 1);
       if (grid.z)
-        hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, true>), grid, dim3(p.W * 64),
+        hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, true, false>), grid, dim3(p.W * 64),
                            3 * TQ * 64 * sizeof(float), stream, a);
       grid.z = a.nchunk;
-      hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, false>), grid, dim3(p.W * 64), shm, stream, a);
+      if (N == p.W * NS)
+        hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, false, false>), grid, dim3(p.W * 64), shm, stream, a);
+      else
+        hipLaunchKernelGGL((ssm::scan_bwd_k<E, V, IT, NS, TQ, false, true>), grid, dim3(p.W * 64), shm, stream, a);
     });
     hipLaunchKernelGGL((ssm::bc_grad_k<E>), dim3(ceil_div(rows * 2 * N < (1l << 22) ? rows * 2 * N : (1l << 22), 256)),
                        dim3(256), 0, stream, a.pbc, nblk, rows, N, (E*)db, (E*)dc);

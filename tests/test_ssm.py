@@ -595,7 +595,7 @@ def _mask(shape, dev, *at):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kw", [{}, {"skip": False, "z": False}, {"skip": False}])
-@pytest.mark.parametrize("n", [4, 8, 16, 40])
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 9, 16, 33, 40])
 def test_selective_scan_infinite_input_gpu(cuda, n, kw):
     """An infinite input gives infinities, not NaN, and only in what it reaches (with maps and skip of one sign, so that
     no infinities of opposite signs meet)."""
