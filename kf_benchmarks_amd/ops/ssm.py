@@ -291,8 +291,11 @@ def selective_scan_reference(x, delta, A, B, C, D=None, z=None, delta_bias=None,
     h = xs.new_zeros((Bn, A.shape[0], Dn)) if initial_state is None else initial_state.to(A.dtype)
     ys = []
     for t in range(T):
-        h = torch.exp(dt[t][:, None] * A) * h + (dt[t] * xs[t])[:, None] * bs[t][:, :, None]
-        ys.append((h * cs[t][:, :, None]).sum(1))
+        on = inside[t][:, :, None]  # (a gradient of zero times an infinite state is not zero)
+        new = torch.exp(dt[t][:, None] * A) * torch.where(on, h, zero) + \
+            (dt[t] * xs[t])[:, None] * bs[t][:, :, None]
+        h = torch.where(on, new, h)
+        ys.append((torch.where(on, h, zero) * cs[t][:, :, None]).sum(1))
     y = torch.stack(ys)
     if D is not None:
         y = y + D * xs

@@ -623,3 +623,36 @@ def test_selective_scan_infinite_input_gpu(cuda, n, kw):
         s = torch.sigmoid(z)
         assert torch.equal(got["z"][after].double(), INF * dy[after].double() * (s * (1 + z * (1 - s))))
     assert (got["state_out"][0, :, 3] == INF).all()
+
+
+def _infinite_last_input(dev, n, state_grad):
+    """What stands behind a sequence's end, in its tile or in padding, adds nothing, not even zero times infinity."""
+    T, B, D = 37, 2, 72
+    i, dy, dh = scan_inputs(T, B, D, n, torch.float32, dev)
+    dh = dh if state_grad else None
+    i["lengths"] = torch.tensor([20, 37], dtype=torch.int32, device=dev)
+    clean = scan_run(i, dy, dh)
+    i["x"] = i["x"].clone()
+    i["x"][19, 0, 3], i["x"][36, 1, 7] = INF, -INF
+    got = scan_run(i, dy, dh)
+    at, rows, ch = ((19, 0, 3), (36, 1, 7)), ((19, 0), (36, 1)), (3, 7)
+    m = lambda *s: _mask(s, dev)  # noqa: E731
+    bad = {"y": _mask((T, B, D), dev, *at), "x": m(T, B, D), "delta": _mask((T, B, D), dev, *at),
+           "z": _mask((T, B, D), dev, *at), "A": m(n, D), "B": _mask((T, B, n), dev, *rows),
+           "C": _mask((T, B, n), dev, *rows), "D": _mask((D,), dev, *ch), "bias": _mask((D,), dev, *ch),
+           "state_out": _mask((B, n, D), dev, (0, slice(None), 3), (1, slice(None), 7))}
+    for k, v in got.items():
+        assert torch.equal(~torch.isfinite(v), bad[k]), k
+        assert torch.equal(v[~bad[k]], clean[k][~bad[k]]), k
+
+
+@pytest.mark.parametrize("state_grad", [True, False])
+def test_selective_scan_infinite_last_input_cpu(state_grad):
+    _infinite_last_input("cpu", 5, state_grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 5, 16, 40])
+@pytest.mark.parametrize("state_grad", [True, False])
+def test_selective_scan_infinite_last_input_gpu(cuda, n, state_grad):
+    _infinite_last_input(cuda, n, state_grad)
