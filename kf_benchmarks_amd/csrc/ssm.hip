@@ -192,7 +192,9 @@ __device__ __forceinline__ float step_size(float raw, bool softplus) {
 }
 
 // h over ``n`` chunks j = from, from + by, ...: h = exp(A sum dt_j) h + end_j,
-// eight chunks' values in flight.
+// eight chunks' values in flight.  The decays of a chunk may multiply to zero where no single one
+// is zero, and zero times an infinite h is NaN: 2^-149 in its place leaves infinities as they are
+// and at most 2^-21 of the largest finite h.
 template <int NS>
 __device__ __forceinline__ void join(const Args& a, int b, int dc, long bnd, long bn, int ns,
                                      const float (&A2)[NS], int from, int by, int n, float (&h)[NS]) {
@@ -211,7 +213,7 @@ __device__ __forceinline__ void join(const Args& a, int b, int dc, long bnd, lon
       if (j0 + q < n)
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-          if (i < ns) h[i] = fmaf(__builtin_amdgcn_exp2f(sum[q] * A2[i]), h[i], end[q][i]);
+          if (i < ns) h[i] = fmaf(fmaxf(__builtin_amdgcn_exp2f(sum[q] * A2[i]), 0x1p-149f), h[i], end[q][i]);
   }
 }
 

@@ -656,3 +656,16 @@ def test_selective_scan_infinite_last_input_cpu(state_grad):
 @pytest.mark.parametrize("state_grad", [True, False])
 def test_selective_scan_infinite_last_input_gpu(cuda, n, state_grad):
     _infinite_last_input(cuda, n, state_grad)
+
+
+@pytest.mark.gpu
+def test_selective_scan_infinite_state_over_chunks_gpu(cuda):
+    """An infinite state stays infinite where the decays of a whole chunk multiply to zero."""
+    T, D, n, t = 1500, 64, 16, 100
+    i, _, _ = scan_inputs(T, 1, D, n, torch.float32, cuda, z=False, skip=False)
+    i["A"], i["B"], i["C"] = 8 * i["A"], i["B"].abs(), i["C"].abs()
+    i["x"][t, 0, 3] = INF
+    with torch.no_grad():
+        got = scan_run(i)
+    assert torch.equal(~torch.isfinite(got["y"]), _mask((T, 1, D), cuda, (slice(t, None), 0, 3)))
+    assert (got["y"][t:, 0, 3] == INF).all() and (got["state_out"][0, :, 3] == INF).all()
