@@ -272,7 +272,11 @@ KFB_API hipError_t kfb_seqlock_check(const long long* seq, long long expect, int
     }
   }
   if (w) {
-    const hipError_t e = hipLaunchHostFunc(stream, copy_word, w);
+    // (a captured host call would be repeated with an argument that its first run frees)
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    hipError_t e = hipStreamIsCapturing(stream, &capture);
+    if (e == hipSuccess && capture != hipStreamCaptureStatusNone) e = hipErrorStreamCaptureUnsupported;
+    if (e == hipSuccess) e = hipLaunchHostFunc(stream, copy_word, w);
     if (e != hipSuccess) {
       delete w;
       return e;
@@ -282,19 +286,12 @@ KFB_API hipError_t kfb_seqlock_check(const long long* seq, long long expect, int
   return hipGetLastError();
 }
 
-// Makes host memory p readable by kfb_seqlock_check; *dev receives the address to
-// give it.  An error is returned and not left behind, where the thread's next
-// launch, of whoever it is, would report it as its own.
-KFB_API hipError_t kfb_host_register(void* p, size_t bytes, void** dev) {
+// Gives host memory p a page-locked copy that kfb_seqlock_check brings up to date; *dev
+// receives the address to give it.
+KFB_API hipError_t kfb_host_stage(void* p, size_t bytes, void** dev) {
   if (!p || !bytes || !dev) return hipErrorInvalidValue;
-  hipError_t e = hipHostRegister(p, bytes, hipHostRegisterMapped);
-  if (e == hipSuccess) {
-    if ((e = hipHostGetDevicePointer(dev, p, 0)) == hipSuccess) return e;
-    (void)hipHostUnregister(p);
-  }
-  (void)hipGetLastError();
   Staged m{(char*)p, nullptr, nullptr, bytes};
-  e = hipHostMalloc((void**)&m.pinned, bytes, hipHostMallocMapped);
+  hipError_t e = hipHostMalloc((void**)&m.pinned, bytes, hipHostMallocMapped);
   if (e == hipSuccess && (e = hipHostGetDevicePointer((void**)&m.dev, m.pinned, 0)) != hipSuccess)
     (void)hipHostFree(m.pinned);
   if (e != hipSuccess) {
@@ -306,6 +303,20 @@ KFB_API hipError_t kfb_host_register(void* p, size_t bytes, void** dev) {
   staged.push_back(m);
   *dev = m.dev;
   return hipSuccess;
+}
+
+// Makes host memory p readable by kfb_seqlock_check: page-locked, or staged.  An error is
+// returned and not left behind, where the thread's next launch, of whoever it is, would
+// report it as its own.
+KFB_API hipError_t kfb_host_register(void* p, size_t bytes, void** dev) {
+  if (!p || !bytes || !dev) return hipErrorInvalidValue;
+  hipError_t e = hipHostRegister(p, bytes, hipHostRegisterMapped);
+  if (e == hipSuccess) {
+    if ((e = hipHostGetDevicePointer(dev, p, 0)) == hipSuccess) return e;
+    (void)hipHostUnregister(p);
+  }
+  (void)hipGetLastError();
+  return kfb_host_stage(p, bytes, dev);
 }
 
 // (waits for checks under way, which still read p)

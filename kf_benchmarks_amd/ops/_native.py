@@ -69,6 +69,7 @@ _SIGS = {
     "kfb_tape_raw_launches": [P],
     "kfb_tape_set_raw": [I],
     "kfb_host_register": [P, ctypes.c_size_t, P],
+    "kfb_host_stage": [P, ctypes.c_size_t, P],
     "kfb_host_unregister": [P],
     "kfb_ipc_export": [P, P, P],
     "kfb_ipc_handle_bytes": [],

@@ -350,3 +350,41 @@ def test_refused_host_registration_leaves_no_error(cuda):
         N.call("kfb_host_register", None, 0, ctypes.byref(dev))
     x.fill_(3.0)
     assert float(x.sum()) == 24.0
+
+
+def _header_word(tmp_path):
+    """(mapping, address, file) of 64 bytes of existing memory, as a peer's header is."""
+    import ctypes
+    import mmap
+    path = tmp_path / "header"
+    path.write_bytes(b"\0" * 64)
+    f = open(path, "r+b")
+    m = mmap.mmap(f.fileno(), 64)
+    return m, ctypes.addressof(ctypes.c_char.from_buffer(m)), f
+
+
+def test_seqlock_check_of_a_staged_word_is_not_captured(cuda, tmp_path):
+    """Where memory cannot be page-locked, a check enqueues a host call: a graph that would repeat it is refused."""
+    import ctypes
+    import torch
+    from kf_benchmarks_amd.ops import _native as N
+    m, host, f = _header_word(tmp_path)
+    dev, words = ctypes.c_void_p(), torch.zeros(2, dtype=torch.int32, device=cuda)
+    N.call("kfb_host_stage", host, 64, ctypes.byref(dev))
+    x = torch.zeros(4, device=cuda)
+    torch.cuda.synchronize()
+
+    def check():
+        N.call("kfb_seqlock_check", dev.value, 0, words.data_ptr(), words.data_ptr() + 4, N.stream(cuda))
+
+    check()
+    with pytest.raises(N.NativeError):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            x.add_(1)
+            check()
+    check()
+    torch.cuda.synchronize()
+    assert words.tolist() == [1, 0]
+    N.call("kfb_host_unregister", host)
+    m.close()
+    f.close()
