@@ -388,3 +388,34 @@ def test_seqlock_check_of_a_staged_word_is_not_captured(cuda, tmp_path):
     N.call("kfb_host_unregister", host)
     m.close()
     f.close()
+
+
+@pytest.mark.parametrize("entry", ["kfb_host_stage", "kfb_host_register"])
+def test_staged_words_follow_the_host(cuda, tmp_path, entry):
+    """A check sees what the host wrote before it; unregistering ends it, a second time is refused; and no refusal on the
+    way (of page-locking memory that exists, or that is registered already) is left for the next launch to report."""
+    import ctypes
+    import struct
+    import torch
+    from kf_benchmarks_amd.ops import _native as N
+    m, host, f = _header_word(tmp_path)
+    devs, x = [ctypes.c_void_p(), ctypes.c_void_p()], torch.zeros(8, device=cuda)
+    ok, torn = (torch.zeros(1, dtype=torch.int32, device=cuda) for _ in range(2))
+    for d in devs:
+        N.call(entry, host, 64, ctypes.byref(d))
+        N.call("kfb_nonfinite", x.data_ptr(), 8, ok.data_ptr(), N.stream(cuda))  # reports a left error as its own
+    seen = []
+    for k, word in ((2, 0), (4, 1), (6, 7)):
+        struct.pack_into("<q", m, 8 * word, k)
+        for d in devs:
+            for expect in (k, k + 1):
+                N.call("kfb_seqlock_check", d.value + 8 * word, expect, ok.data_ptr(), torn.data_ptr(), N.stream(cuda))
+                seen.append(int(ok))
+    assert seen == [1, 0] * 6 and int(torn) == 6
+    for d in devs:
+        N.call("kfb_host_unregister", host)
+    with pytest.raises(N.NativeError):
+        N.call("kfb_host_unregister", host)
+    N.call("kfb_nonfinite", x.data_ptr(), 8, ok.data_ptr(), N.stream(cuda))
+    m.close()
+    f.close()
