@@ -109,15 +109,18 @@ class _Header:
         host, dev = self._dev[r]
         return None if dev is None else dev + 8 * word
 
+    # mappings that the device may still read: never unmapped
+    _held = []
+
     def close(self):
         if self._dev:
             from ..ops import _native as N
-            for host, dev in self._dev.values():
+            for r, (host, dev) in self._dev.items():
                 if host is not None:
                     try:
                         N.call("kfb_host_unregister", host)
                     except N.NativeError:
-                        pass
+                        _Header._held.append(self._maps.pop(r))
             self._dev = {}
         for f, m in self._maps.values():
             m.close()
