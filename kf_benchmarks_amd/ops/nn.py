@@ -671,8 +671,8 @@ def on_device(x):
 _SAME_DEVICE = contextlib.nullcontext()
 
 
-N.register_optional("kfb_gn_fwd_ws", [N.I, N.L, N.L, N.I, N.I], N.L)
-N.register_optional("kfb_gn_bwd_ws", [N.I, N.L, N.L, N.I, N.I], N.L)
+N.register_optional("kfb_gn_fwd_ws", [N.I, N.L, N.L, N.I, N.I, N.I], N.L)
+N.register_optional("kfb_gn_bwd_ws", [N.I, N.L, N.L, N.I, N.I, N.I], N.L)
 N.register_optional("kfb_gn_fwd", [N.I, N.P, N.P, N.L, N.L, N.I, N.I, N.P, N.P, N.F, N.I, N.P, N.P,
                                    N.P, N.P])
 N.register_optional("kfb_gn_bwd", [N.I, N.P, N.P, N.P, N.L, N.L, N.I, N.I, N.P, N.P, N.I, N.P, N.P,
@@ -684,10 +684,11 @@ def _gn_forward(x, gamma, beta, groups, eps, act):
     hw = x.numel() // (n * C)
     dt = N.dt(x)
     y = torch.empty_like(x)
-    st = x.new_empty((2 * n * groups + size_query("kfb_gn_fwd_ws", dt, n, hw, C, groups),),
-                     dtype=torch.float32)
+    px, py = x.data_ptr(), y.data_ptr()
+    ws = size_query("kfb_gn_fwd_ws", dt, n, hw, C, groups, (px | py) & 15)
+    st = x.new_empty((2 * n * groups + ws,), dtype=torch.float32)
     base = st.data_ptr()
-    N.call("kfb_gn_fwd", dt, x.data_ptr(), y.data_ptr(), n, hw, C, groups, N.ptr(gamma),
+    N.call("kfb_gn_fwd", dt, px, py, n, hw, C, groups, N.ptr(gamma),
            N.ptr(beta), eps, act, base, base + 4 * n * groups, base + 8 * n * groups,
            N.stream(x.device))
     return y, st
@@ -712,7 +713,8 @@ class _GroupNorm(torch.autograd.Function):
         hw = x.numel() // (n * C)
         dx = torch.empty_like(x)
         grads, acc = grad_buffers(ctx.params)
-        ws = x.new_empty((size_query("kfb_gn_bwd_ws", N.dt(x), n, hw, C, groups),),
+        at = (x.data_ptr() | dy.data_ptr() | dx.data_ptr()) & 15
+        ws = x.new_empty((size_query("kfb_gn_bwd_ws", N.dt(x), n, hw, C, groups, at),),
                          dtype=torch.float32)
         base = st.data_ptr()
         N.call("kfb_gn_bwd", N.dt(x), dy.data_ptr(), x.data_ptr(), dx.data_ptr(), n, hw, C, groups,

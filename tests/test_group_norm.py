@@ -242,3 +242,20 @@ def test_group_norm_refuses_other_types_gpu(cuda):
     (g,) = torch.autograd.grad(F.group_norm(x, None, None, 2).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [N.BF16, N.F32])
+@pytest.mark.parametrize("C,groups", [(4096, 1), (2048, 1), (4096, 8), (8192, 1), (1600, 8)])
+@pytest.mark.parametrize("at", [0, 4])
+def test_workspace_does_not_grow_with_the_rows(dtype, C, groups, at):
+    """At most 2048 slabs of 2 C channel sums for any number of rows, wide groups and unaligned tensors among them."""
+    for rows in (1, 1000, 32768, 1 << 24):
+        assert 0 < N.query("kfb_gn_bwd_ws", dtype, rows, 1, C, groups, at) <= 2048 * 2 * C
+        assert N.query("kfb_gn_fwd_ws", dtype, rows, 1, C, groups, at) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups,dtype", [((2100, 2052), 1, torch.float32), ((2060, 4104), 1, torch.bfloat16),
+                                                ((1100, 2, 1026), 2, torch.float16), ((1030, 8208), 2, torch.bfloat16)])
+def test_group_norm_more_images_than_slabs_gpu(cuda, shape, groups, dtype):
+    compare(shape, groups, "silu", dtype, cuda)
