@@ -307,6 +307,25 @@ __global__ void __launch_bounds__(256) step_k(Args a, T* __restrict__ state) {
   store_vec<T, V>((T*)a.y + (long)b * a.D + c, u);
 }
 
+// y [T][B][D] = x with the rows at or past each sequence's length zero, whatever they
+// hold: a wave a row.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) mask_rows_k(const T* __restrict__ x, long ldx, const int* __restrict__ len,
+                                                   T* __restrict__ y, long rows, int B, int D) {
+  for (long row = (long)blockIdx.x * 4 + threadIdx.x / 64; row < rows; row += (long)gridDim.x * 4) {
+    const bool on = row / B < len[row % B];
+    for (int c = threadIdx.x % 64 * V; c < D; c += 64 * V) {
+      Raw<T, V> v;
+      float f[V];
+      if (on) v.load(x + row * ldx + c);
+      else v.zero();
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] = v[k];
+      store_vec<T, V>(y + row * D + c, f);
+    }
+  }
+}
+
 inline bool bad(const Args& a) {
   return a.T <= 0 || a.B <= 0 || a.D <= 0 || a.K < 1 || a.K > KMAX;
 }
@@ -415,6 +434,17 @@ KFB_API hipError_t kfb_cconv_step(int dtype, int vec, const void* x, long ldx, v
       hipLaunchKernelGGL((cconv::step_k<E, V, KIND>), dim3(ceil_div((long)D / V * B, 256)), dim3(256),
                          0, stream, a, (E*)state);
     });
+  }));
+  return hipGetLastError();
+}
+
+KFB_API hipError_t kfb_mask_rows(int dtype, int vec, const void* x, long ldx, const int* len, void* y,
+                                 int T, int B, int D, hipStream_t stream) {
+  if (T <= 0 || B <= 0 || D <= 0 || !len) return hipErrorInvalidValue;
+  const long rows = (long)T * B, wgs = (rows + 3) / 4;
+  KFB_DISPATCH_DTYPE(dtype, E, KFB_CCONV_VEC(vec, 16 / sizeof(E), V, {
+    hipLaunchKernelGGL((cconv::mask_rows_k<E, V>), dim3((unsigned)(wgs < 65536 ? wgs : 65536)), dim3(256), 0,
+                       stream, (const E*)x, ldx, len, (E*)y, rows, B, D);
   }));
   return hipGetLastError();
 }

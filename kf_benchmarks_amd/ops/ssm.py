@@ -43,6 +43,7 @@ N.register_optional("kfb_cconv_fwd", [_I, _I, _P, _L] + [_P] * 6 + [_I] * 6 + [_
 N.register_optional("kfb_cconv_bwd", [_I, _I] + [_P, _L] * 2 + [_P] * 9 + [_I] * 2 + [_P] + [_I] * 6
                     + [_P])
 N.register_optional("kfb_cconv_step", [_I, _I, _P, _L] + [_P] * 4 + [_I] * 4 + [_P])
+N.register_optional("kfb_mask_rows", [_I, _I, _P, _L, _P, _P] + [_I] * 3 + [_P])
 
 MAX_STATES, MAX_TAPS = 64, 8
 
@@ -507,6 +508,44 @@ def split_columns(x, widths):
     return _SplitColumns.apply(x.contiguous(), tuple(widths))
 
 
+def _masked(x, lengths):
+    x, ld = _rows(x)
+    T, B, D = x.shape
+    y = torch.empty((T, B, D), dtype=x.dtype, device=x.device)
+    N.call("kfb_mask_rows", N.dt(x), int(_vec(D, 16 // x.element_size(), (x, ld))), x.data_ptr(), ld,
+           lengths.data_ptr(), y.data_ptr(), T, B, D, N.stream(x.device))
+    return y
+
+
+class _MaskRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, lengths):
+        ctx.save_for_backward(lengths)
+        return _masked(x, lengths)
+
+    @staticmethod
+    @F_ops.first_order
+    def backward(ctx, dy):
+        return _masked(dy, ctx.saved_tensors[0]), None
+
+
+def mask_rows(x, lengths):
+    """x [T, B, D] with the rows at or past each sequence's length zero, whatever
+    they hold (a product's weight gradient would multiply them by zero, which NaN
+    and infinities survive)."""
+    if x.dim() != 3 or x.numel() == 0:
+        raise ValueError("mask_rows: a non-empty [T, B, D] tensor expected, got %s" % (tuple(x.shape),))
+    _check_lengths(x, lengths)
+    if lengths is None:
+        return x
+    if not x.is_cuda:
+        inside = torch.arange(x.shape[0], device=x.device)[:, None] < lengths
+        return torch.where(inside[..., None], x, torch.zeros((), dtype=x.dtype, device=x.device))
+    N.dt(x)
+    with F_ops.on_device(x):
+        return _MaskRows.apply(x, lengths) if _needs_grad(x) else _masked(x, lengths)
+
+
 def ssm_layer(x, w_in, conv_w, conv_b, w_rank, w_delta, w_bc, delta_bias, A_log, D, norm_w,
               groups=1, lengths=None, reverse=False, low=None):
     """One selective state space layer of x [T, B, din] -> [T, B, E]:
@@ -517,7 +556,8 @@ def ssm_layer(x, w_in, conv_w, conv_b, w_rank, w_delta, w_bc, delta_bias, A_log,
 
     w_in [din, 2 E], conv_w [K, E], w_rank [E, R], w_delta [R, E], w_bc [E, 2 N], A_log
     [N, E] (fp32 masters in the TF layout); ``low``: compute-type copies of the
-    four matrices by name."""
+    four matrices by name.  Rows past ``lengths`` count nowhere and give zero."""
+    x = mask_rows(x, lengths)
     T, B, din = x.shape
     E, Ns = conv_w.shape[1], A_log.shape[0]
     low = low or {}

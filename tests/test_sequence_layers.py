@@ -421,3 +421,61 @@ def test_forward_mode_tangents_are_refused_gpu(cuda, grad):
             with pytest.raises(ValueError):
                 call()
         F.group_norm(x, None, None, 2)
+
+
+def _layer_with_poisoned_padding(dev, reverse):
+    """What padding holds counts in no output and in no gradient of the layer, its first projection's among them."""
+    T, B, din, E = 20, 4, 24, 32
+    p = {k: v.to(dev) for k, v in layer_params(din, E).items()}
+    g = torch.Generator().manual_seed(1)
+    x, dy = (torch.randn(T, B, n, generator=g).to(dev) for n in (din, E))
+    lengths = torch.tensor([20, 3, 17, 0], dtype=torch.int32, device=dev)
+    behind = torch.arange(T, device=dev)[:, None] >= lengths
+    runs = []
+    for fill in (0.0, float("nan"), float("inf")):
+        x[behind] = fill
+        runs.append(run_layer(x, p, dy, lengths=lengths, reverse=reverse))
+    assert all(torch.isfinite(t).all() for t in runs[0])
+    for run in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+    assert (runs[0][0][behind] == 0).all() and (runs[0][1][behind] == 0).all()
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_layer_with_poisoned_padding_cpu(reverse):
+    _layer_with_poisoned_padding("cpu", reverse)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_layer_with_poisoned_padding_gpu(cuda, reverse):
+    _layer_with_poisoned_padding(cuda, reverse)
+
+
+def _mask_rows(dev, dtype, D, wide):
+    T, B = 7, 5
+    x = torch.randn(T, B, wide).to(dtype).to(dev)[..., wide - D:].detach().requires_grad_()
+    lengths = torch.tensor([7, 0, 3, -2, 9], dtype=torch.int32, device=dev)
+    behind = torch.arange(T, device=dev)[:, None] >= lengths
+    with torch.no_grad():
+        x[behind] = float("nan")
+    y = ssm.mask_rows(x, lengths)
+    dy = torch.randn(T, B, D).to(dtype).to(dev)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for got, of in ((y, x), (dx, dy), (ssm.mask_rows(x.detach(), lengths), x)):
+        assert (got[behind] == 0).all() and torch.equal(got[~behind], of[~behind])
+    assert ssm.mask_rows(x, None) is x
+    for bad in (lengths[:4], lengths.long()):
+        with pytest.raises(ValueError):
+            ssm.mask_rows(x, bad)
+
+
+def test_mask_rows_cpu():
+    _mask_rows("cpu", torch.float32, 6, 9)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,wide", [(1, 1), (8, 8), (7, 30), (520, 1040), (1600, 1600)])
+def test_mask_rows_gpu(cuda, dtype, D, wide):
+    _mask_rows(cuda, dtype, D, wide)
