@@ -259,3 +259,39 @@ def test_workspace_does_not_grow_with_the_rows(dtype, C, groups, at):
                                                 ((1100, 2, 1026), 2, torch.float16), ((1030, 8208), 2, torch.bfloat16)])
 def test_group_norm_more_images_than_slabs_gpu(cuda, shape, groups, dtype):
     compare(shape, groups, "silu", dtype, cuda)
+
+
+FAR = [((1, 40, 40, 64), 8), ((2, 56, 56, 64), 32), ((6, 7, 7, 64), 8), ((200, 256), 8), ((3, 9, 2052), 1)]
+
+
+def far_inputs(shape, groups):
+    """Inputs whose groups' means are 1000 and more of their standard deviations."""
+    x, gamma, beta, dy = inputs(shape, groups, None, torch.float32, "cpu", offset=0.0)
+    g = torch.Generator().manual_seed(2)
+    x = x + 3000.0 * (1 + 0.2 * torch.rand(groups, generator=g)).repeat_interleave(shape[-1] // groups)
+    v = x.double().reshape(shape[0], -1, groups, shape[-1] // groups)
+    assert (v.mean((1, 3)).abs() / v.std((1, 3))).min() > 1000
+    return x, gamma, beta, dy
+
+
+@pytest.mark.parametrize("shape,groups", FAR)
+def test_far_mean_tells_variances_apart(shape, groups):
+    """The bound passes the variance of centred fp32 values and not the mean square minus the squared mean."""
+    x, gamma, beta, _ = far_inputs(shape, groups)
+    v = x.reshape(shape[0], -1, groups, shape[-1] // groups)
+    mu = v.mean((1, 3), keepdim=True)
+    want = oracle(x, None, None, groups, 1e-5, None)["y"]
+    centred = ((v - mu) ** 2).mean((1, 3), keepdim=True)
+    one_pass = (v * v).mean((1, 3), keepdim=True) - mu * mu
+    check(((v - mu) / torch.sqrt(centred + 1e-5)).reshape(shape), want, "y")
+    with pytest.raises(AssertionError):
+        check(((v - mu) / torch.sqrt(one_pass.clamp(min=0) + 1e-5)).reshape(shape), want, "y")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", FAR)
+def test_group_norm_of_far_means_gpu(cuda, shape, groups):
+    x, gamma, beta, dy = (t.to(cuda) for t in far_inputs(shape, groups))
+    want = oracle(x, gamma, beta, groups, 1e-5, None, dy)
+    for name, t in run(x, gamma, beta, groups, None, dy).items():
+        check(t, want[name], name)
