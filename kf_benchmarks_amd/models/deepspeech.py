@@ -185,7 +185,7 @@ class DeepSpeech2(nn.Module):
         self.conv2 = _ConvBN(32, 32, (21, 11), (2, 1), (10, 5), gen, device)
         f = (feature_bins + 10 - 11) // 2 + 1
         f = (f + 10 - 11) // 1 + 1
-        kind = rnn_ops._KIND.get(rnn_type)
+        kind = None if rnn_type == "ssm" else rnn_ops._KIND[rnn_type]
         dirs = 2 if bidirectional else 1
         self.rnns = nn.ModuleList()
         self.bns = nn.ModuleList()

@@ -479,3 +479,10 @@ def test_mask_rows_cpu():
 @pytest.mark.parametrize("D,wide", [(1, 1), (8, 8), (7, 30), (520, 1040), (1600, 1600)])
 def test_mask_rows_gpu(cuda, dtype, D, wide):
     _mask_rows(cuda, dtype, D, wide)
+
+
+def test_deepspeech2_names_an_unknown_layer_type():
+    from kf_benchmarks_amd.models.deepspeech import DeepSpeech2
+    for layers in (0, 1):
+        with pytest.raises(KeyError, match="bogus"):
+            DeepSpeech2(29, layers, "bogus", True, 8, True, 161, torch.Generator(), "cpu")
