@@ -481,6 +481,28 @@ def test_mask_rows_gpu(cuda, dtype, D, wide):
     _mask_rows(cuda, dtype, D, wide)
 
 
+@pytest.mark.parametrize("bidirectional", [True, False])
+def test_deepspeech2_ssm_trains_cpu(bidirectional):
+    """The network is built of selective state space layers, and a step reaches every parameter of each direction."""
+    from kf_benchmarks_amd import datasets, params as P
+    from kf_benchmarks_amd.models import model_config
+    from kf_benchmarks_amd.models.deepspeech import _SSMLayer
+    from kf_benchmarks_amd.models.model import make_network
+    d = datasets.create_dataset(None, "librispeech")
+    m = model_config.get_model_config("deepspeech2", d, P.make_params(model="deepspeech2"))
+    m.max_time_steps, m.max_label_length, m.rnn_hidden_size, m.num_rnn_layers = 60, 8, 16, 2
+    m.rnn_type, m.is_bidirectional = "ssm", bidirectional
+    m.set_batch_size(2)
+    net = make_network(m, d.num_classes, "cpu", torch.float32)
+    inputs = m.get_synthetic_inputs("x", d.num_classes, "cpu", 0)
+    loss = m.loss_function(inputs, net.forward_inputs(inputs))
+    loss.backward()
+    assert torch.isfinite(loss) and sum(isinstance(k, _SSMLayer) for k in net.modules()) == 2
+    got = {n: p.grad for n, p in net.named_parameters() if n.rsplit(".", 1)[-1][:-2] in LAYER}
+    assert len(got) == 2 * (1 + bidirectional) * len(LAYER)
+    assert all(g is not None and torch.isfinite(g).all() and g.abs().sum() > 0 for g in got.values())
+
+
 def test_deepspeech2_names_an_unknown_layer_type():
     from kf_benchmarks_amd.models.deepspeech import DeepSpeech2
     for layers in (0, 1):
