@@ -366,8 +366,6 @@ using namespace kfb;
     default: { constexpr int KP = 8; constexpr bool EXACT = false; __VA_ARGS__; break; } \
   }
 
-KFB_API int kfb_cconv_max_taps() { return cconv::KMAX; }
-
 KFB_API long kfb_cconv_bwd_ws(int T, int B, int D, int K) {
   if (T <= 0 || B <= 0 || D <= 0 || K <= 0) return 0;
   return (long)cconv::bwd_slabs(T, B, D, cconv::run_of(T, (long)ceil_div(D, cconv::BV) * B)) * (K + 1) * D;

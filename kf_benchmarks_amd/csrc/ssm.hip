@@ -856,8 +856,6 @@ using namespace kfb;
     default: { constexpr int NS = 8, TQ = 8; KFB_SSM_VEC(v, V, IT, 2, __VA_ARGS__) break; }                \
   }
 
-KFB_API int kfb_ssm_max_states() { return 64; }
-
 // Floats of: the fp32 copy of B and C and the forward's chunk ends (what = 0),
 // the saved states of a training forward (1), the backward's workspace (2).
 KFB_API long kfb_ssm_floats(int what, int T, int B, int D, int N) {

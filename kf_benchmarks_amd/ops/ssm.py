@@ -30,14 +30,12 @@ from . import _native as N
 from . import nn as F_ops
 
 _I, _L, _P = N.I, N.L, N.P
-N.register_optional("kfb_ssm_max_states", [])
 N.register_optional("kfb_ssm_floats", [_I] * 5, _L)
 N.register_optional("kfb_ssm_furthest_state", [_I] * 4, _L)
 N.register_optional("kfb_ssm_scan_fwd", [_I, _I] + [_P, _L] * 5 + [_P] * 9 + [_I] * 7 + [_P])
 N.register_optional("kfb_ssm_scan_bwd", [_I, _I] + [_P, _L] * 4 + [_P] * 16 + [_I] * 3 + [_P] +
                     [_I] * 7 + [_P])
 N.register_optional("kfb_ssm_step", [_I] + [_P, _L] * 5 + [_P] * 5 + [_I] * 5 + [_P])
-N.register_optional("kfb_cconv_max_taps", [])
 N.register_optional("kfb_cconv_bwd_ws", [_I] * 4, _L)
 N.register_optional("kfb_cconv_fwd", [_I, _I, _P, _L] + [_P] * 6 + [_I] * 6 + [_P])
 N.register_optional("kfb_cconv_bwd", [_I, _I] + [_P, _L] * 2 + [_P] * 9 + [_I] * 2 + [_P] + [_I] * 6
