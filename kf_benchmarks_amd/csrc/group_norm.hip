@@ -19,8 +19,9 @@
 //     56 x 256 bf16 in 32 groups, 51 MB a tensor: statistics 13.7 us, y 23.6,
 //     backward sums 22.5, dx 35.0 (3.8, 4.3, 4.6 and 4.4 TB/s; a copy: 5.2);
 //   * rows (group_norm_rows.hip): one row an image, groups held by lanes;
-//   * gn_*_any_k: one workgroup per group, for groups wider than 512 vectors
-//     (every image and group of the split case above this way: 480 us, not 95).
+//   * gn_*_any_k: one workgroup per image and group (backward: up to 2048, each a
+//     slab of channel sums), for groups wider than 512 vectors (every image and
+//     group of the split case above this way: 480 us, not 95).
 #include "group_norm.h"
 
 namespace kfb {

@@ -8,7 +8,8 @@
 // row loaded while one is worked on.  8192 waves, one row at a time: 22.2 us for
 // 13984 rows of 1600 bf16 values in 8 groups (4.0 TB/s; a copy reaches 5.2);
 // 4096 waves took 25.3 us, two rows at a time 25.1, 16384 waves (each reads gamma
-// and beta, as many bytes as its rows) 33.6.
+// and beta, as many bytes as its rows) 33.6.  With SiLU 28 us forward and 53 us backward
+// (134 MB of x, dy and dx: 2.6 TB/s), and 7 us for the channel sums.
 #include "group_norm.h"
 
 namespace kfb {

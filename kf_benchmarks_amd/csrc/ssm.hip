@@ -18,12 +18,16 @@
 //
 // Bound by the vector units: an exponential (8 cycles a wave) and four fused
 // operations (4 cycles each) per state, 24 cycles, and about 60 operations a value
-// around it; the bytes take a quarter to a half of that.  With 16 states 874 x 64 x
-// 1600 bf16 values take 460 us, 5.1 ps each, two thirds of the vector units' rate
-// (of the rest, the walks' scalar loads and barriers have most).  Where B D / 64 workgroups do not fill the card, a sequence is
-// cut into chunks: ends_k walks every chunk but the last from a zero state, and
-// because the decays of a chunk multiply to exp(A sum dt), the state before a
-// chunk follows from the earlier chunks' (end, sum dt) alone.
+// around it; the bytes take a quarter to a half of that.  By its counters the walk of 874 x
+// 16 x 1600 bf16 values with 16 states (115 us) keeps them busy for 83% of its time.
+// Where B D / 64 workgroups do not fill the card, a sequence is cut into chunks: a first
+// launch (ENDS, 73 us there, 72% busy) walks every chunk but the last from a zero state,
+// and because the decays of a chunk multiply to exp(A sum dt), the state before a chunk
+// follows from the earlier chunks' (end, sum dt) alone.
+//
+// Zeros that stand for nothing are selected, not multiplied by: a missing skip, the states
+// that a wave does not have, the rows behind a sequence's end.  An infinite input then
+// gives infinities where the formulas do, and in nothing else.
 #include "act.h"
 #include "raw.h"
 
@@ -430,7 +434,7 @@ template <int M> __device__ __forceinline__ int lane_value(int l) {
 // atomics, the same sums on every run.  Bound by the vector units too: 70
 // instructions a step of 4 states (19 of them the sums over lanes), 1840 a wave and tile,
 // at two waves a SIMD (H and dec take 128 registers): 874 x 16 x 1600 values take
-// 500 us.  Tiles of 8 steps (three waves a SIMD), decays computed again instead of
+// 519 us, the vector units busy for 52% of it.  Tiles of 8 steps (three waves a SIMD), decays computed again instead of
 // kept, and two states a wave were no faster (550 to 890 us).
 // ENDS: only the gradient before each chunk, from zero behind it, and sum dt.
 // PART: as in scan_fwd_k (and all tiles in the loop for the last ones: fewer kernels).
@@ -762,8 +766,8 @@ param_grad_k(const float* __restrict__ p, int S, int N, int D, const float* log_
 }
 
 // One token: state [B][N][D] in place.  64 channels x 4 waves, wave w the
-// states w, w + 4, ...  64 x 16 x 1600 states, 13 MB read and written: 5.8 us
-// (2.3 TB/s: short of work for the card's 256 units, and the launch is 3.5).
+// states w, w + 4, ...  64 x 16 x 1600 states, 13 MB read and written: 6.0 us
+// (2.2 TB/s; an empty launch alone is 3.5).
 template <typename T>
 __global__ void __launch_bounds__(256) step_k(Args a, float* __restrict__ state) {
   __shared__ float yp[4][64];
