@@ -669,3 +669,23 @@ def test_selective_scan_infinite_state_over_chunks_gpu(cuda):
         got = scan_run(i)
     assert torch.equal(~torch.isfinite(got["y"]), _mask((T, 1, D), cuda, (slice(t, None), 0, 3)))
     assert (got["y"][t:, 0, 3] == INF).all() and (got["state_out"][0, :, 3] == INF).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [2, 4, 6])
+def test_causal_conv_infinite_gradient_gpu(cuda, K):
+    """An infinite gradient of y gives infinities, not NaN, and only in what it reaches, wherever in a run it stands."""
+    T, B, D = 64, 2, 24
+    i, dy, _ = conv_inputs(T, B, D, K, torch.float32, cuda, act=None)
+    i["x"], i["w"] = i["x"].abs() + 0.1, i["w"].abs() + 0.1
+    clean = conv_run(i, dy)
+    for t in range(K, 20):
+        bad = dy.clone()
+        bad[t, 1, 5] = INF
+        got = conv_run(i, bad)
+        dx, dw, db = (torch.zeros_like(got[k], dtype=torch.bool) for k in ("x", "w", "b"))
+        dx[t - K + 1:t + 1, 1, 5] = True
+        dw[:, 5] = True
+        db[5] = True
+        for k, m in (("x", dx), ("w", dw), ("b", db)):
+            assert (got[k][m] == INF).all() and torch.equal(got[k][~m], clean[k][~m]), (t, k)
