@@ -18,7 +18,7 @@ namespace kfb {
 namespace cconv {
 
 // most taps; positions whose loads are in flight together, forward and backward
-// (backward with 8: 216 registers, 62 us for 874 x 16 x 1600 bf16, with 4: 162, 45 us)
+// (backward with 8: 216 registers, 62 us for 874 x 16 x 1600 bf16, with 4: 158, 44 us)
 constexpr int KMAX = 8, UF = 8, UB = 4;
 
 struct Args {

@@ -231,7 +231,7 @@ __device__ __forceinline__ float zero_from(float v, int s, int len) {
 // so that no wait for a load waits for a store just issued.
 // ENDS: only the state after each chunk, from zero, and the chunk's sum of dt.
 // PART: not every wave has NS states; those that it does not have stay zero by selection
-// (zero times an infinite input is not).  (ENDS stores none of them.)
+// (zero times an infinite input or gradient is not).  (ENDS stores none of them.)
 template <typename T, int V, int IT, int NS, int TQ, bool ENDS, bool PART>
 __global__ void __launch_bounds__(512) scan_fwd_k(Args a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(512) scan_bwd_k(Args a) {
           float p = 0.f, q = 0.f, red[2 * NS];
 #pragma unroll
           for (int i = 0; i < NS; ++i) {
-            const float g = fmaf(bc.C(k, i), e, carry[i]);
+            const float full = fmaf(bc.C(k, i), e, carry[i]), g = PART && i >= ns ? 0.f : full;
             p = fmaf(g, bc.B(k, i), p);
             red[i] = g * u.y;
             red[NS + i] = e * H[r][i];

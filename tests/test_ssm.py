@@ -689,3 +689,26 @@ def test_causal_conv_infinite_gradient_gpu(cuda, K):
         db[5] = True
         for k, m in (("x", dx), ("w", dw), ("b", db)):
             assert (got[k][m] == INF).all() and torch.equal(got[k][~m], clean[k][~m]), (t, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 3, 4, 5, 8, 9, 16, 33, 40])
+def test_selective_scan_infinite_gradient_gpu(cuda, n):
+    """An infinite gradient of y gives infinities, not NaN, and only in what it reaches (inputs, maps and skip of one sign)."""
+    T, B, D, t = 37, 2, 72, 20
+    i, dy, dh = scan_inputs(T, B, D, n, torch.float32, cuda, state=True, z=False)
+    for k in ("x", "B", "C", "D", "state"):
+        i[k] = i[k].abs()
+    clean = scan_run(i, dy, dh)
+    dy = dy.clone()
+    dy[t, 0, 3] = INF
+    got = scan_run(i, dy, dh)
+    before, ch, m = (slice(0, t + 1), 0, 3), (slice(None), 3), lambda *s: _mask(s, cuda)  # noqa: E731
+    bad = {"y": m(T, B, D), "state_out": m(B, n, D), "x": _mask((T, B, D), cuda, before), "delta": _mask((T, B, D), cuda, before),
+           "A": _mask((n, D), cuda, ch), "B": _mask((T, B, n), cuda, (slice(0, t + 1), 0)), "C": _mask((T, B, n), cuda, (t, 0)),
+           "D": _mask((D,), cuda, 3), "bias": _mask((D,), cuda, 3), "state": _mask((B, n, D), cuda, (0, slice(None), 3))}
+    for k, v in got.items():
+        assert torch.equal(~torch.isfinite(v), bad[k]), k
+        assert torch.equal(v[~bad[k]], clean[k][~bad[k]]), k
+    for k in ("x", "B", "C", "D", "state"):
+        assert (got[k][bad[k]] == INF).all(), k
