@@ -223,7 +223,7 @@ def causal_conv(x, w, b=None, activation=None, lengths=None, initial_state=None,
     if T > 1 << 20:
         raise ValueError("causal_conv: at most 2^20 rows, got %d" % T)
     if initial_state is not None:
-        initial_state = initial_state.contiguous() if K > 1 else None
+        initial_state = initial_state.contiguous()  # (of one tap: empty, and its gradient too)
     with F_ops.on_device(x):
         if _needs_grad(x, w, b, initial_state):
             return _CausalConv.apply(x, w, b, initial_state, lengths, act, bool(reverse),

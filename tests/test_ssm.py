@@ -712,3 +712,9 @@ def test_selective_scan_infinite_gradient_gpu(cuda, n):
         assert torch.equal(v[~bad[k]], clean[k][~bad[k]]), k
     for k in ("x", "B", "C", "D", "state"):
         assert (got[k][bad[k]] == INF).all(), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [{}, {"ragged": True, "poison": True}, {"state_grad": False, "reverse": True}])
+def test_causal_conv_of_one_tap_with_its_empty_state_gpu(cuda, kw):
+    conv_compare(9, 3, 24, 1, torch.bfloat16, cuda, state=True, **kw)
