@@ -7,7 +7,8 @@ constant size (csrc/ssm.hip, csrc/causal_conv.hip).
   * ``selective_scan``  - the recurrence, its skip and its gate;
   * ``causal_conv_step`` / ``selective_scan_step`` - one token, the state
     updated in place;
-  * ``ssm_layer``       - one layer: projections, convolution, scan, group norm.
+  * ``ssm_layer``       - one layer: projections, convolution, scan, group norm;
+  * ``mask_rows``       - zero past each sequence's length, in front of a product.
 
 Activations may be fp32, bf16 or fp16 and column slices of a wider
 [T, B, ...] tensor (a projection's output): they are read in place.  Parameters
